@@ -47,8 +47,9 @@ enum kvq_status {
 /* Library version: major*10000 + minor*100 + patch. kvq_version() returns
  * the version the library was built as; a binding declares the argument lists
  * of one major version and must refuse a library of another. 2.0.0 added the
- * capacity argument of kvq_quantize (1.x had none). */
-#define KVQ_VERSION 20000
+ * capacity argument of kvq_quantize (1.x had none), 2.1.0 tree attention, key
+ * weights and eviction. */
+#define KVQ_VERSION 20100
 int kvq_version(void);
 
 /* Thread-local message describing the last error on this thread ("" if none). */
@@ -418,6 +419,120 @@ int kvq_prefill_attn_paged(const void* q, int q_dtype, const int64_t* q_strides,
                            int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
                            int64_t group_size, int64_t Sk, int is_causal, float sm_scale,
                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * kvq_tree_attn — attention of a block of T drafted tokens that form a tree,
+ * over a cache that already holds their rows (appended last, as for a causal
+ * block): query row i attends every key before the block, and of the block's
+ * own T keys (a sequence's last T) those t with mask[b][i][t] != 0. No
+ * reference counterpart (its attention masks causally,
+ * kernels/llama3/attention_quant.py:91-97).
+ *
+ * mask: bytes, element strides mask_strides[3] = (b, i, t), 0 where shared.
+ * seq_lens (device int32 [B], may be NULL): keys of each sequence, the block's
+ * rows among them, clamped to [0, Sk]; NULL: Sk for all. A sequence shorter
+ * than T holds the block's last rows only. A row that attends no key is zero;
+ * a key that a row does not attend does not reach it, whatever it holds.
+ * q, out: [B, Hq, T, D] of q_dtype, element strides [4]. Any dtype, group size
+ * and D <= 256 (KVQ_EUNSUP above).
+ * workspace: uninitialised scratch of kvq_tree_attn_workspace_bytes (16-byte
+ * aligned) lets a launch split over the keys; without it the call is right but
+ * slower. Calls that overlap in time must not share it.
+ */
+int kvq_tree_attn(const void* q, int q_dtype, const int64_t* q_strides,
+                  const void* k_packed, const int64_t* kp_strides,
+                  const void* k_scales, const int64_t* ks_strides,
+                  const void* v_packed, const int64_t* vp_strides,
+                  const void* v_scales, const int64_t* vs_strides, int scale_dtype,
+                  const void* mask, const int64_t* mask_strides,
+                  void* out, const int64_t* out_strides,
+                  int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t group_size,
+                  const int32_t* seq_lens, int64_t Sk, float sm_scale,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+int64_t kvq_tree_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D,
+                                      int64_t group_size, int64_t Sk, int q_dtype, int scale_dtype);
+
+/* kvq_tree_attn over a paged cache (Sk <= table_cols * page_size). A key whose
+ * page has no block is not attended. */
+int kvq_tree_attn_paged(const void* q, int q_dtype, const int64_t* q_strides,
+                        const void* k_pool, const int64_t* kp_strides,
+                        const void* k_scale_pool, const int64_t* ks_strides,
+                        const void* v_pool, const int64_t* vp_strides,
+                        const void* v_scale_pool, const int64_t* vs_strides, int scale_dtype,
+                        const int32_t* block_table, int64_t table_stride, int64_t table_cols,
+                        int64_t num_blocks, int64_t page_size,
+                        const void* mask, const int64_t* mask_strides,
+                        void* out, const int64_t* out_strides,
+                        int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t group_size,
+                        const int32_t* seq_lens, int64_t Sk, float sm_scale,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * kvq_add_key_weights — adds to weights[b][kvh][j] (fp32, element strides
+ * weight_strides[3]) the softmax weights that the block's Sq query rows give
+ * key j, summed over the KV head's query heads and the rows; keys past a
+ * sequence's length keep theirs. kvq_attn_key_weights also writes the block's
+ * attention to out. Causal blocks align bottom-right, as kvq_decode_attn. No
+ * reference counterpart. The sums' order is fixed (no atomics). A row that
+ * attends no key, or whose softmax is not finite, adds nothing.
+ * workspace: kvq_key_weights_workspace_bytes of uninitialised scratch, 16-byte
+ * aligned (needed: KVQ_ESPACE without). Calls that overlap must not share it.
+ */
+int kvq_attn_key_weights(const void* q, int q_dtype, const int64_t* q_strides,
+                         const void* k_packed, const int64_t* kp_strides,
+                         const void* k_scales, const int64_t* ks_strides,
+                         const void* v_packed, const int64_t* vp_strides,
+                         const void* v_scales, const int64_t* vs_strides, int scale_dtype,
+                         void* out, const int64_t* out_strides,
+                         float* weights, const int64_t* weight_strides,
+                         int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int64_t group_size,
+                         const int32_t* seq_lens, int64_t Sk, int is_causal, float sm_scale,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+int kvq_add_key_weights(const void* q, int q_dtype, const int64_t* q_strides,
+                        const void* k_packed, const int64_t* kp_strides,
+                        const void* k_scales, const int64_t* ks_strides, int scale_dtype,
+                        float* weights, const int64_t* weight_strides,
+                        int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int64_t group_size,
+                        const int32_t* seq_lens, int64_t Sk, int is_causal, float sm_scale,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+int64_t kvq_key_weights_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
+                                        int64_t group_size, int64_t Sk, int q_dtype, int scale_dtype,
+                                        int with_attention);
+
+/*
+ * kvq_select_keys — the rows an eviction keeps: index[b][h][0 .. n_keep)
+ * (int32, contiguous) gets, ascending, the first `sink` and last `recent` of
+ * the sequence's keys and, of the others, those of the greatest weight. Equal
+ * weights go to the lowest row, NaN ranks above every number. A sequence of at
+ * most n_keep keys keeps all; -1 fills the rest. seq_lens as kvq_tree_attn.
+ */
+int kvq_select_keys(const float* weights, const int64_t* weight_strides, int64_t B, int64_t H, int64_t S,
+                    const int32_t* seq_lens, int64_t n_keep, int64_t sink, int64_t recent,
+                    int32_t* index, void* stream);
+
+/*
+ * kvq_move_rows — row index[b][h][i] of each of 1 to 5 tensors becomes row
+ * first + i of its destination (first: device int32 [B], or first0). Strides
+ * are (batch, head, row) in bytes, three per tensor; a row is row_bytes
+ * contiguous bytes. index strides in elements (0 where shared). An index
+ * outside [0, S) and a destination outside [0, dst_rows) move nothing. With
+ * in_place != 0 (src and dst the same memory) any index is right, up to 64 KiB
+ * of rows per tensor and head (KVQ_EINVAL above); otherwise they must not
+ * overlap. kvq_move_rows_paged moves in place between a paged cache's
+ * positions; strides are (head, row) in bytes, and a position whose page has
+ * no block moves nothing.
+ */
+int kvq_move_rows(int64_t n_tensors, const void* const* src, const int64_t* src_strides,
+                  void* const* dst, const int64_t* dst_strides, const int64_t* row_bytes,
+                  const int32_t* index, const int64_t* index_strides,
+                  int64_t B, int64_t H, int64_t S, int64_t n, int64_t dst_rows,
+                  const int32_t* first, int64_t first0, int in_place, void* stream);
+int kvq_move_rows_paged(int64_t n_tensors, void* const* pools, const int64_t* pool_strides,
+                        const int64_t* row_bytes,
+                        const int32_t* block_table, int64_t table_stride, int64_t table_cols,
+                        int64_t num_blocks, int64_t page_size,
+                        const int32_t* index, const int64_t* index_strides,
+                        int64_t B, int64_t H, int64_t n, const int32_t* first, int64_t first0, void* stream);
 
 #ifdef __cplusplus
 }

@@ -414,12 +414,198 @@ FN(py_prefill_attn_paged) {
                               s[4], s[5], s[6], (int)s[7], f, ws, wb[0], st));
 }
 
+/* (B, Hq, Hkv, T, D, G, Sk, q_dtype, scale_dtype) -> workspace bytes of tree_attn */
+FN(py_tree_plan) {
+  WANT(9);
+  INTS(s, 0, 9);
+  return PyLong_FromLongLong(
+      kvq_tree_attn_workspace_bytes(s[0], s[1], s[2], s[3], s[4], s[5], s[6], (int)s[7], (int)s[8]));
+}
+
+/* (q, q_dtype, k_packed, k_scales, v_packed, v_scales, scale_dtype, mask, out, B, Hq, Hkv, T, D, G, seq_lens, Sk,
+   sm_scale, workspace, workspace_bytes, stream) */
+FN(py_tree_attn) {
+  WANT(21);
+  TENSOR(q, 0, 4);
+  INTS(qd, 1, 1);
+  TENSOR(kp, 2, 3);
+  TENSOR(ks, 3, 3);
+  TENSOR(vp, 4, 3);
+  TENSOR(vs, 5, 3);
+  INTS(sd, 6, 1);
+  TENSOR(m, 7, 3);
+  TENSOR(o, 8, 4);
+  INTS(s, 9, 6);
+  POINTER(sl, 15);
+  INTS(n, 16, 1);
+  FLOAT(f, 17);
+  POINTER(ws, 18);
+  INTS(wb, 19, 1);
+  POINTER(st, 20);
+  CALL(kvq_tree_attn(q.p, (int)qd[0], q.st, kp.p, kp.st, ks.p, ks.st, vp.p, vp.st, vs.p, vs.st, (int)sd[0], m.p, m.st,
+                     o.p, o.st, s[0], s[1], s[2], s[3], s[4], s[5], (const int32_t *)sl, n[0], f, ws, wb[0], st));
+}
+
+/* (q, q_dtype, k_pool, k_scales, v_pool, v_scales, scale_dtype, table, mask, out, B, Hq, Hkv, T, D, G, seq_lens, Sk,
+   sm_scale, workspace, workspace_bytes, stream) */
+FN(py_tree_attn_paged) {
+  WANT(22);
+  TENSOR(q, 0, 4);
+  INTS(qd, 1, 1);
+  TENSOR(kp, 2, 2);
+  TENSOR(ks, 3, 2);
+  TENSOR(vp, 4, 2);
+  TENSOR(vs, 5, 2);
+  INTS(sd, 6, 1);
+  TABLE(t, 7);
+  TENSOR(m, 8, 3);
+  TENSOR(o, 9, 4);
+  INTS(s, 10, 6);
+  POINTER(sl, 16);
+  INTS(n, 17, 1);
+  FLOAT(f, 18);
+  POINTER(ws, 19);
+  INTS(wb, 20, 1);
+  POINTER(st, 21);
+  CALL(kvq_tree_attn_paged(q.p, (int)qd[0], q.st, kp.p, kp.st, ks.p, ks.st, vp.p, vp.st, vs.p, vs.st, (int)sd[0],
+                           (const int32_t *)t.bt, t.g[0], t.g[1], t.g[2], t.g[3], m.p, m.st, o.p, o.st, s[0], s[1],
+                           s[2], s[3], s[4], s[5], (const int32_t *)sl, n[0], f, ws, wb[0], st));
+}
+
+/* (B, Hq, Hkv, Sq, D, G, Sk, q_dtype, scale_dtype, with attention) -> workspace bytes */
+FN(py_key_weights_plan) {
+  WANT(10);
+  INTS(s, 0, 10);
+  return PyLong_FromLongLong(kvq_key_weights_workspace_bytes(s[0], s[1], s[2], s[3], s[4], s[5], s[6], (int)s[7],
+                                                             (int)s[8], (int)s[9]));
+}
+
+/* (q, q_dtype, k_packed, k_scales, v_packed, v_scales, scale_dtype, out, weights, B, Hq, Hkv, Sq, D, G, seq_lens, Sk,
+   causal, sm_scale, workspace, workspace_bytes, stream) */
+FN(py_attn_key_weights) {
+  WANT(22);
+  TENSOR(q, 0, 4);
+  INTS(qd, 1, 1);
+  TENSOR(kp, 2, 3);
+  TENSOR(ks, 3, 3);
+  TENSOR(vp, 4, 3);
+  TENSOR(vs, 5, 3);
+  INTS(sd, 6, 1);
+  TENSOR(o, 7, 4);
+  TENSOR(w, 8, 3);
+  INTS(s, 9, 6);
+  POINTER(sl, 15);
+  INTS(n, 16, 2);
+  FLOAT(f, 18);
+  POINTER(ws, 19);
+  INTS(wb, 20, 1);
+  POINTER(st, 21);
+  CALL(kvq_attn_key_weights(q.p, (int)qd[0], q.st, kp.p, kp.st, ks.p, ks.st, vp.p, vp.st, vs.p, vs.st, (int)sd[0],
+                            o.p, o.st, (float *)w.p, w.st, s[0], s[1], s[2], s[3], s[4], s[5], (const int32_t *)sl,
+                            n[0], (int)n[1], f, ws, wb[0], st));
+}
+
+/* (q, q_dtype, k_packed, k_scales, scale_dtype, weights, B, Hq, Hkv, Sq, D, G, seq_lens, Sk, causal, sm_scale,
+   workspace, workspace_bytes, stream) */
+FN(py_add_key_weights) {
+  WANT(19);
+  TENSOR(q, 0, 4);
+  INTS(qd, 1, 1);
+  TENSOR(kp, 2, 3);
+  TENSOR(ks, 3, 3);
+  INTS(sd, 4, 1);
+  TENSOR(w, 5, 3);
+  INTS(s, 6, 6);
+  POINTER(sl, 12);
+  INTS(n, 13, 2);
+  FLOAT(f, 15);
+  POINTER(ws, 16);
+  INTS(wb, 17, 1);
+  POINTER(st, 18);
+  CALL(kvq_add_key_weights(q.p, (int)qd[0], q.st, kp.p, kp.st, ks.p, ks.st, (int)sd[0], (float *)w.p, w.st, s[0], s[1],
+                           s[2], s[3], s[4], s[5], (const int32_t *)sl, n[0], (int)n[1], f, ws, wb[0], st));
+}
+
+/* (weights, B, H, S, seq_lens, n_keep, sink, recent, index, stream) */
+FN(py_select_keys) {
+  WANT(10);
+  TENSOR(w, 0, 3);
+  INTS(s, 1, 3);
+  POINTER(sl, 4);
+  INTS(k, 5, 3);
+  TENSOR(x, 8, 3);
+  POINTER(st, 9);
+  CALL(kvq_select_keys((const float *)w.p, w.st, s[0], s[1], s[2], (const int32_t *)sl, k[0], k[1], k[2],
+                       (int32_t *)x.p, st));
+}
+
+/* Pointers and n byte strides of each of a tuple's tensors (sizes: a tuple of their element sizes). */
+static int read_tensors(PyObject *o, PyObject *sizes, Py_ssize_t most, Py_ssize_t n, void **p, int64_t *st) {
+  if (!PyTuple_Check(o) || !PyTuple_Check(sizes) || PyTuple_GET_SIZE(o) != PyTuple_GET_SIZE(sizes) ||
+      PyTuple_GET_SIZE(o) > most) {
+    PyErr_Format(PyExc_ValueError, "expected tuples of at most %zd tensors and of their element sizes", most);
+    return -1;
+  }
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(o); ++i) {
+    tensor_arg a;
+    const int64_t size = PyLong_AsLongLong(PyTuple_GET_ITEM(sizes, i));
+    if (size == -1 && PyErr_Occurred()) return -1;
+    if (read_tensor(PyTuple_GET_ITEM(o, i), &a, n) < 0) return -1;
+    p[i] = a.p;
+    for (Py_ssize_t k = 0; k < n; ++k) st[n * i + k] = a.st[k] * size;
+  }
+  return (int)PyTuple_GET_SIZE(o);
+}
+
+static int read_widths(PyObject *o, int64_t *w, Py_ssize_t n) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != n) {
+    PyErr_SetString(PyExc_ValueError, "expected a row's bytes for each tensor");
+    return -1;
+  }
+  return read_ints(&PyTuple_GET_ITEM(o, 0), n, w);
+}
+
+/* (sources, destinations, element sizes, row bytes, index, B, H, S, n, dst_rows, first, first0, in_place, stream) */
+FN(py_move_rows) {
+  WANT(14);
+  void *src[5], *dst[5];
+  int64_t ss[15], ds[15], w[5];
+  const int k = read_tensors(args[0], args[2], 5, 3, src, ss);
+  if (k < 0 || read_tensors(args[1], args[2], 5, 3, dst, ds) < 0 || read_widths(args[3], w, k) < 0) return NULL;
+  TENSOR(x, 4, 3);
+  INTS(s, 5, 5);
+  POINTER(fp, 10);
+  INTS(f, 11, 2);
+  POINTER(st, 13);
+  CALL(kvq_move_rows(k, (const void *const *)src, ss, dst, ds, w, (const int32_t *)x.p, x.st, s[0], s[1], s[2], s[3],
+                     s[4], (const int32_t *)fp, f[0], (int)f[1], st));
+}
+
+/* (pools, element sizes, row bytes, table, index, B, H, n, first, first0, stream) */
+FN(py_move_rows_paged) {
+  WANT(11);
+  void *p[5];
+  int64_t ps[10], w[5];
+  const int k = read_tensors(args[0], args[1], 5, 2, p, ps);
+  if (k < 0 || read_widths(args[2], w, k) < 0) return NULL;
+  TABLE(t, 3);
+  TENSOR(x, 4, 3);
+  INTS(s, 5, 3);
+  POINTER(fp, 8);
+  INTS(f, 9, 1);
+  POINTER(st, 10);
+  CALL(kvq_move_rows_paged(k, p, ps, w, (const int32_t *)t.bt, t.g[0], t.g[1], t.g[2], t.g[3], (const int32_t *)x.p,
+                           x.st, s[0], s[1], s[2], (const int32_t *)fp, f[0], st));
+}
+
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {
     ENTRY(quantize),          ENTRY(quantize_kv),    ENTRY(quantize_paged),    ENTRY(quantize_kv_paged),
     ENTRY(dequantize),        ENTRY(dequantize_paged), ENTRY(plan),            ENTRY(decode_attn),
     ENTRY(decode_attn_paged), ENTRY(decode_step),    ENTRY(decode_step_paged), ENTRY(prefill_attn),
-    ENTRY(prefill_attn_paged), {NULL, NULL, 0, NULL}};
+    ENTRY(prefill_attn_paged), ENTRY(tree_plan),     ENTRY(tree_attn),         ENTRY(tree_attn_paged),
+    ENTRY(key_weights_plan),  ENTRY(attn_key_weights), ENTRY(add_key_weights), ENTRY(select_keys),
+    ENTRY(move_rows),         ENTRY(move_rows_paged), {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvq_host", "libkvint4.so's entry points, taking tensors.",
                                     -1, methods, NULL, NULL, NULL, NULL};

@@ -52,6 +52,15 @@ EXPORTED_SYMBOLS = (
     "kvq_prefill_attn_workspace_bytes",
     "kvq_prefill_attn_staged_workspace_bytes",
     "kvq_prefill_attn_paged",
+    "kvq_tree_attn",
+    "kvq_tree_attn_workspace_bytes",
+    "kvq_tree_attn_paged",
+    "kvq_attn_key_weights",
+    "kvq_add_key_weights",
+    "kvq_key_weights_workspace_bytes",
+    "kvq_select_keys",
+    "kvq_move_rows",
+    "kvq_move_rows_paged",
 )
 
 _lock = threading.Lock()
@@ -186,6 +195,42 @@ def _declare(lib: ctypes.CDLL) -> None:
         _i64, _i64, _i64, _i64, _i64,
         _vp, _i64, ctypes.c_float,
         _i64, _vp, _i64, _vp,
+    ]
+    lib.kvq_tree_attn_workspace_bytes.restype = _i64
+    lib.kvq_tree_attn_workspace_bytes.argtypes = [_i64] * 7 + [_i32, _i32]
+    cache = [_vp, _i64p, _vp, _i64p]
+    lib.kvq_tree_attn.restype = _i32
+    lib.kvq_tree_attn.argtypes = [
+        _vp, _i32, _i64p, *cache, *cache, _i32, _vp, _i64p, _vp, _i64p,
+        _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, ctypes.c_float, _vp, _i64, _vp,
+    ]
+    lib.kvq_tree_attn_paged.restype = _i32
+    lib.kvq_tree_attn_paged.argtypes = [
+        _vp, _i32, _i64p, *cache, *cache, _i32, *pg, _vp, _i64p, _vp, _i64p,
+        _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, ctypes.c_float, _vp, _i64, _vp,
+    ]
+    lib.kvq_key_weights_workspace_bytes.restype = _i64
+    lib.kvq_key_weights_workspace_bytes.argtypes = [_i64] * 7 + [_i32, _i32, _i32]
+    lib.kvq_attn_key_weights.restype = _i32
+    lib.kvq_attn_key_weights.argtypes = [
+        _vp, _i32, _i64p, *cache, *cache, _i32, _vp, _i64p, _vp, _i64p,
+        _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i32, ctypes.c_float, _vp, _i64, _vp,
+    ]
+    lib.kvq_add_key_weights.restype = _i32
+    lib.kvq_add_key_weights.argtypes = [
+        _vp, _i32, _i64p, *cache, _i32, _vp, _i64p,
+        _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i32, ctypes.c_float, _vp, _i64, _vp,
+    ]
+    lib.kvq_select_keys.restype = _i32
+    lib.kvq_select_keys.argtypes = [_vp, _i64p, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp]
+    ptrs = ctypes.POINTER(_vp)
+    lib.kvq_move_rows.restype = _i32
+    lib.kvq_move_rows.argtypes = [
+        _i64, ptrs, _i64p, ptrs, _i64p, _i64p, _vp, _i64p, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp,
+    ]
+    lib.kvq_move_rows_paged.restype = _i32
+    lib.kvq_move_rows_paged.argtypes = [
+        _i64, ptrs, _i64p, _i64p, *pg, _vp, _i64p, _i64, _i64, _i64, _vp, _i64, _vp,
     ]
 
 

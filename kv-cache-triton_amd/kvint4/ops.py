@@ -1017,3 +1017,409 @@ def decode_step_paged(
         )
     nat.check(rc, "kvq_decode_step_paged")
     return out
+
+
+# ---------------------------------------------------------------------------
+# trees of drafted tokens, key weights, eviction
+
+
+def _check_cache(what: str, q: torch.Tensor, caches: tuple, B: int, Hkv: int, D: int, group_size: int) -> None:
+    """Argument checks of the contiguous cache tensors (codes, scales, ...) of
+    an operator whose queries are q [B, Hq, Sq, D]."""
+    if group_size < 1:
+        raise ValueError("group_size must be > 0")
+    if Hkv < 1 or q.shape[1] % Hkv:
+        raise ValueError(f"the query heads ({q.shape[1]}) must be a multiple of n_kv_heads ({Hkv})")
+    S = caches[0].shape[2] if caches[0].dim() == 4 else -1
+    for codes, scales in zip(caches[0::2], caches[1::2]):
+        if codes.dim() != 4 or scales.dim() != 4 or codes.shape[:3] != (B, Hkv, S) or scales.shape[:3] != (B, Hkv, S):
+            raise ValueError(f"{what}: codes and scales must be [B={B}, n_kv_heads={Hkv}, Sk, .] of one Sk "
+                             f"(got {tuple(codes.shape)}, {tuple(scales.shape)})")
+        if codes.dtype != torch.uint8 or scales.dtype not in SUPPORTED_FLOATS or scales.dtype != caches[1].dtype:
+            raise ValueError(f"{what}: codes must be uint8, scales bf16/fp16/fp32 of one dtype")
+        if codes.shape[-1] < packed_width(D, group_size) or scales.shape[-1] < num_groups(D, group_size):
+            raise ValueError(f"{what}: cache last dims are too small for this head dim / group size")
+        if codes.stride(-1) != 1 or scales.stride(-1) != 1:
+            raise ValueError(f"{what}: cache last dims must be contiguous")
+
+
+def _check_block(what: str, q: torch.Tensor, out: torch.Tensor | None, *others: torch.Tensor) -> torch.Tensor:
+    """The output of an operator of queries q [B, Hq, Sq, D] on the device that
+    holds every operand: `out`, or a new tensor."""
+    if q.dim() != 4 or q.dtype not in SUPPORTED_FLOATS:
+        raise ValueError(f"{what}: q must be [B, Hq, Sq, D] in bf16/fp16/fp32")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"{what}: out must have q's shape and dtype")
+    _check_cuda(q, out, *others, what=what)
+    for t in (out, *others):
+        if t.get_device() != q.get_device():
+            raise ValueError(f"{what}: every tensor must be on q's device ({q.device}; got one on {t.device})")
+    return out
+
+
+def _lens_ptr(what: str, seq_lens: torch.Tensor | None, B: int, device: torch.device) -> tuple:
+    """(pointer or None, the tensor behind it) of per-sequence lengths."""
+    if seq_lens is None:
+        return None, None
+    if seq_lens.dtype != torch.int32 or not seq_lens.is_cuda or seq_lens.numel() != B:
+        raise ValueError(f"{what}: seq_lens must be a device int32 tensor of shape [B]")
+    if seq_lens.device != device:
+        raise ValueError(f"{what}: seq_lens must be on the operands' device ({device}; got {seq_lens.device})")
+    seq_lens = seq_lens.contiguous()
+    return seq_lens.data_ptr(), seq_lens
+
+
+def _scratch(nbytes: int, what: str, device: torch.device) -> tuple:
+    """(tensor, pointer, bytes) of uninitialised scratch for one call: from the
+    caching allocator, and back to it with the call (under graph capture: the
+    graph's own pool), so that no two graphs share it."""
+    if nbytes < 0:
+        nat.check(nbytes, what)
+    if nbytes == 0:
+        return None, None, 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), nbytes
+
+
+def _tree_mask(mask: torch.Tensor, B: int, T: int) -> torch.Tensor:
+    """tree_mask as bytes [B, T, T] (one for the batch: stride 0)."""
+    if mask.dtype != torch.bool or mask.shape not in ((T, T), (B, T, T)):
+        raise ValueError(f"tree_mask must be bool [{T}, {T}] or [{B}, {T}, {T}] (got {mask.dtype} {tuple(mask.shape)})")
+    return mask.view(torch.uint8).expand(B, T, T)
+
+
+def tree_attention(
+    q: torch.Tensor,
+    k_packed: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_packed: torch.Tensor,
+    v_scales: torch.Tensor,
+    tree_mask: torch.Tensor,
+    *,
+    n_kv_heads: int,
+    group_size: int,
+    sm_scale: float,
+    seq_lens: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of a tree of T drafted tokens, q [B, Hq, T, D], over a cache
+    that holds their rows already: the last T of each sequence's Sk rows (or of
+    its first seq_lens[b], a device int32 [B]), as for a causal block. Draft i
+    attends every row before the block, and of the block those t with
+    tree_mask[i, t] ([T, T], or [B, T, T] for a tree per sequence): its
+    ancestors and itself. A draft that attends no row gives zeros; a row that
+    it does not attend has no effect on it, whatever that row holds. Any float
+    dtypes and group size, D up to 256 (KVQUnsupported above)."""
+    what = "tree_attention"
+    out = _check_block(what, q, out, k_packed, k_scales, v_packed, v_scales, tree_mask)
+    B, Hq, T, D = q.shape
+    _check_cache(what, q, (k_packed, k_scales, v_packed, v_scales), B, n_kv_heads, D, group_size)
+    mask = _tree_mask(tree_mask, B, T)
+    Sk = k_packed.shape[2]
+    sl_ptr, seq_lens = _lens_ptr(what, seq_lens, B, q.device)
+    qd, sd = nat.DTYPE_CODE[q.dtype], nat.DTYPE_CODE[k_scales.dtype]
+    with nat.device_of(q) as stream:
+        ws, ws_ptr, ws_len = _scratch(nat.host().tree_plan(B, Hq, n_kv_heads, T, D, group_size, Sk, qd, sd),
+                                      "kvq_tree_attn_workspace_bytes", q.device)
+        rc = nat.host().tree_attn(
+            q, qd, k_packed, k_scales, v_packed, v_scales, sd, mask, out, B, Hq, n_kv_heads, T, D, group_size, sl_ptr,
+            Sk, float(sm_scale), ws_ptr, ws_len, stream,
+        )
+    nat.check(rc, "kvq_tree_attn")
+    return out
+
+
+def tree_attention_paged(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_pool: torch.Tensor,
+    v_scales: torch.Tensor,
+    pt: PageTable,
+    tree_mask: torch.Tensor,
+    *,
+    n_kv_heads: int,
+    group_size: int,
+    sm_scale: float,
+    seq_lens: torch.Tensor | None = None,
+    seq_len: int | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """tree_attention over a paged cache: sequence b holds its first
+    seq_lens[b] tokens (device int32 [B]) or `seq_len`, the block's T rows
+    among them. A position whose page has no block is not attended."""
+    what = "tree_attention_paged"
+    out = _check_block(what, q, out, k_pool, k_scales, v_pool, v_scales, pt.table, tree_mask)
+    B, Hq, T, D = q.shape
+    if n_kv_heads < 1 or Hq % n_kv_heads:
+        raise ValueError(f"the query heads ({Hq}) must be a multiple of n_kv_heads ({n_kv_heads})")
+    if group_size < 1:
+        raise ValueError("group_size must be > 0")
+    if pt.table.shape[0] < B:
+        raise ValueError("block table has fewer rows than the batch")
+    for pool, sc in ((k_pool, k_scales), (v_pool, v_scales)):
+        _check_pool(pool, sc, pt, n_kv_heads, D, group_size)
+    if v_scales.dtype != k_scales.dtype:
+        raise ValueError("K and V scale pools must share a dtype")
+    mask = _tree_mask(tree_mask, B, T)
+    sl_ptr, seq_lens = _lens_ptr(what, seq_lens, B, q.device)
+    Sk = pt.capacity
+    if sl_ptr is None:
+        if seq_len is None or not 0 <= int(seq_len) <= Sk:
+            raise ValueError(f"seq_len must be in [0, {Sk}] when seq_lens is not given")
+        Sk = int(seq_len)
+    qd, sd = nat.DTYPE_CODE[q.dtype], nat.DTYPE_CODE[k_scales.dtype]
+    with nat.device_of(q) as stream:
+        ws, ws_ptr, ws_len = _scratch(nat.host().tree_plan(B, Hq, n_kv_heads, T, D, group_size, Sk, qd, sd),
+                                      "kvq_tree_attn_workspace_bytes", q.device)
+        rc = nat.host().tree_attn_paged(
+            q, qd, k_pool, k_scales, v_pool, v_scales, sd, pt.args(), mask, out, B, Hq, n_kv_heads, T, D, group_size,
+            sl_ptr, Sk, float(sm_scale), ws_ptr, ws_len, stream,
+        )
+    nat.check(rc, "kvq_tree_attn_paged")
+    return out
+
+
+def _check_weights(what: str, key_weights: torch.Tensor, B: int, H: int, S: int) -> None:
+    if key_weights.dtype != torch.float32 or key_weights.dim() != 3 or key_weights.shape[:2] != (B, H) \
+            or key_weights.shape[2] < S:
+        raise ValueError(f"{what}: key_weights must be fp32 [B={B}, n_kv_heads={H}, at least {S}] "
+                         f"(got {key_weights.dtype} {tuple(key_weights.shape)})")
+    if B and any(n > 1 and s == 0 for n, s in zip(key_weights.shape, key_weights.stride())):
+        raise ValueError(f"{what}: key_weights must hold a sum of its own for every key (it is a broadcast view)")
+
+
+def add_key_weights(
+    q: torch.Tensor,
+    k_packed: torch.Tensor,
+    k_scales: torch.Tensor,
+    key_weights: torch.Tensor,
+    *,
+    n_kv_heads: int,
+    group_size: int,
+    is_causal: bool,
+    sm_scale: float,
+    seq_lens: torch.Tensor | None = None,
+) -> None:
+    """Add to key_weights [B, n_kv_heads, >= Sk] (fp32, in place) the softmax
+    weights that the queries q [B, Hq, Sq, D] give each cached key, summed over
+    the KV head's query heads and the Sq rows: what an eviction ranks keys by.
+    Causal blocks align bottom-right. Keys past seq_lens[b] keep their sum; a
+    row that attends no key, or whose softmax is not finite, adds nothing."""
+    what = "add_key_weights"
+    _check_block(what, q, q, k_packed, k_scales, key_weights)
+    B, Hq, Sq, D = q.shape
+    _check_cache(what, q, (k_packed, k_scales), B, n_kv_heads, D, group_size)
+    Sk = k_packed.shape[2]
+    _check_weights(what, key_weights, B, n_kv_heads, Sk)
+    sl_ptr, seq_lens = _lens_ptr(what, seq_lens, B, q.device)
+    qd, sd = nat.DTYPE_CODE[q.dtype], nat.DTYPE_CODE[k_scales.dtype]
+    with nat.device_of(q) as stream:
+        ws, ws_ptr, ws_len = _scratch(
+            nat.host().key_weights_plan(B, Hq, n_kv_heads, Sq, D, group_size, Sk, qd, sd, 0),
+            "kvq_key_weights_workspace_bytes", q.device)
+        rc = nat.host().add_key_weights(
+            q, qd, k_packed, k_scales, sd, key_weights, B, Hq, n_kv_heads, Sq, D, group_size, sl_ptr, Sk,
+            1 if is_causal else 0, float(sm_scale), ws_ptr, ws_len, stream,
+        )
+    nat.check(rc, "kvq_add_key_weights")
+
+
+def attention_with_key_weights(
+    q: torch.Tensor,
+    k_packed: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_packed: torch.Tensor,
+    v_scales: torch.Tensor,
+    key_weights: torch.Tensor,
+    *,
+    n_kv_heads: int,
+    group_size: int,
+    is_causal: bool,
+    sm_scale: float,
+    seq_lens: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of q [B, Hq, Sq, D] over the cache (as
+    attention_over_quantized) that also adds its softmax weights to
+    key_weights (as add_key_weights)."""
+    what = "attention_with_key_weights"
+    out = _check_block(what, q, out, k_packed, k_scales, v_packed, v_scales, key_weights)
+    B, Hq, Sq, D = q.shape
+    _check_cache(what, q, (k_packed, k_scales, v_packed, v_scales), B, n_kv_heads, D, group_size)
+    Sk = k_packed.shape[2]
+    _check_weights(what, key_weights, B, n_kv_heads, Sk)
+    sl_ptr, seq_lens = _lens_ptr(what, seq_lens, B, q.device)
+    qd, sd = nat.DTYPE_CODE[q.dtype], nat.DTYPE_CODE[k_scales.dtype]
+    with nat.device_of(q) as stream:
+        ws, ws_ptr, ws_len = _scratch(
+            nat.host().key_weights_plan(B, Hq, n_kv_heads, Sq, D, group_size, Sk, qd, sd, 1),
+            "kvq_key_weights_workspace_bytes", q.device)
+        rc = nat.host().attn_key_weights(
+            q, qd, k_packed, k_scales, v_packed, v_scales, sd, out, key_weights, B, Hq, n_kv_heads, Sq, D, group_size,
+            sl_ptr, Sk, 1 if is_causal else 0, float(sm_scale), ws_ptr, ws_len, stream,
+        )
+    nat.check(rc, "kvq_attn_key_weights")
+    return out
+
+
+def select_keys(
+    key_weights: torch.Tensor,
+    n_keep: int,
+    *,
+    recent: int = 0,
+    sink: int = 0,
+    seq_lens: torch.Tensor | None = None,
+    seq_len: int | None = None,
+) -> torch.Tensor:
+    """The rows that an eviction to n_keep rows keeps, int32 [B, H, n_keep]
+    ascending: of each sequence's keys (its first seq_lens[b], a device int32
+    [B], or `seq_len`, or all) the first `sink`, the last `recent`, and of the
+    others those of the greatest key_weights [B, H, S] (fp32). Equal weights go
+    to the lowest row; NaN ranks above every number. A sequence of at most
+    n_keep keys keeps them all, and -1 fills the rest."""
+    what = "select_keys"
+    if key_weights.dim() != 3:
+        raise ValueError(f"{what}: key_weights must be fp32 [B, H, S]")
+    B, H, S = key_weights.shape
+    if key_weights.dtype != torch.float32:
+        raise ValueError(f"{what}: key_weights must be fp32 (got {key_weights.dtype})")
+    _check_cuda(key_weights, what=what)
+    if seq_len is not None:
+        if not 0 <= int(seq_len) <= S:
+            raise ValueError(f"{what}: seq_len {seq_len} outside [0, {S}]")
+        if seq_lens is not None:
+            raise ValueError(f"{what}: seq_len or seq_lens, not both")
+        S = int(seq_len)
+    n_keep, recent, sink = int(n_keep), int(recent), int(sink)
+    if min(n_keep, recent, sink) < 0 or recent + sink > n_keep:
+        raise ValueError(f"{what}: n_keep ({n_keep}) must hold sink ({sink}) and recent ({recent})")
+    sl_ptr, seq_lens = _lens_ptr(what, seq_lens, B, key_weights.device)
+    index = torch.empty((B, H, n_keep), dtype=torch.int32, device=key_weights.device)
+    with nat.device_of(key_weights) as stream:
+        rc = nat.host().select_keys(key_weights, B, H, S, sl_ptr, n_keep, sink, recent, index, stream)
+    nat.check(rc, "kvq_select_keys")
+    return index
+
+
+def _check_index(what: str, index: torch.Tensor, B: int, H: int, device: torch.device) -> torch.Tensor:
+    """index [B or 1, H or 1, n] as [B, H, n] (stride 0 where shared)."""
+    if index.dtype != torch.int32 or index.dim() != 3 or index.shape[0] not in (1, B) or index.shape[1] not in (1, H):
+        raise ValueError(f"{what}: index must be int32 [B={B} or 1, H={H} or 1, n] (got {index.dtype} "
+                         f"{tuple(index.shape)})")
+    if index.device != device:
+        raise ValueError(f"{what}: index must be on the tensors' device ({device}; got {index.device})")
+    return index.expand(B, H, index.shape[2])
+
+
+def _first(what: str, first, B: int, device: torch.device) -> tuple:
+    """(pointer or None, scalar, the tensor behind the pointer) of the first destination row."""
+    if not isinstance(first, torch.Tensor):
+        if int(first) < 0:
+            raise ValueError(f"{what}: first must be >= 0")
+        return None, int(first), None
+    if first.dtype != torch.int32 or first.numel() != B or first.device != device:
+        raise ValueError(f"{what}: first must be an int or an int32 tensor [B] on the tensors' device")
+    first = first.contiguous()
+    return first.data_ptr(), 0, first
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """[first, last) byte addresses that a tensor's elements lie in."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    n = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (n + 1) * t.element_size()
+
+
+def _row_bytes(t: torch.Tensor) -> int:
+    return t.element_size() * (t.shape[3] if t.dim() == 4 else 1)
+
+
+# Bytes of rows per tensor and head that move in place (the workgroup holds
+# them in LDS between reading and writing).
+MOVE_IN_PLACE_BYTES = 65536
+
+
+def move_rows(tensors, index: torch.Tensor, *, out=None, first=0) -> None:
+    """Row index[b, h, i] of each of up to five tensors [B, H, S, w] or [B, H, S]
+    (a cache's codes and scales, its key weights) becomes row first + i of the
+    tensor's destination: `out`, tensors of the same kinds that overlap none of
+    the sources, or in place (out=None), where at most MOVE_IN_PLACE_BYTES of
+    rows per tensor and head move. index: int32 [B, H, n] (either leading size
+    may be 1: shared). `first`: an int, or an int32 tensor [B]. An index or a
+    destination outside its tensor (an index of -1, say) moves nothing, and
+    rows that nothing moves to are left as they are."""
+    what = "move_rows"
+    tensors = tuple(tensors)
+    if not 1 <= len(tensors) <= 5 or any(t.dim() not in (3, 4) for t in tensors):
+        raise ValueError(f"{what}: 1 to 5 tensors [B, H, S, w] or [B, H, S]")
+    dst = tensors if out is None else tuple(out)
+    if len(dst) != len(tensors):
+        raise ValueError(f"{what}: out must hold a destination for every tensor")
+    _check_cuda(*tensors, *dst, index, what=what)
+    B, H, S = tensors[0].shape[:3]
+    dev, rows = tensors[0].device, dst[0].shape[2] if dst[0].dim() in (3, 4) else -1
+    for t, d in zip(tensors, dst):
+        if t.shape[:3] != (B, H, S) or d.dim() != t.dim() or d.shape[:3] != (B, H, rows) or d.shape[3:] != t.shape[3:] \
+                or d.dtype != t.dtype:
+            raise ValueError(f"{what}: tensors must share [B, H, S], and out's match them but for the rows "
+                             f"(got {tuple(t.shape)} {t.dtype} -> {tuple(d.shape)} {d.dtype})")
+        if t.device != dev or d.device != dev:
+            raise ValueError(f"{what}: every tensor must be on one device")
+        if t.dim() == 4 and (t.stride(3) != 1 or d.stride(3) != 1):
+            raise ValueError(f"{what}: rows must be contiguous")
+    if out is not None:
+        spans = [_span(t) for t in tensors]
+        for d in dst:
+            lo, hi = _span(d)
+            if any(lo < h and l < hi for l, h in spans):
+                raise ValueError(f"{what}: out overlaps the tensors that it is read from")
+    index = _check_index(what, index, B, H, dev)
+    first_ptr, first0, first = _first(what, first, B, dev)
+    n = index.shape[2]
+    if B == 0 or H == 0 or n == 0 or any(_row_bytes(t) == 0 for t in tensors):
+        return
+    with nat.device_of(index) as stream:
+        rc = nat.host().move_rows(
+            tensors, dst, tuple(t.element_size() for t in tensors), tuple(_row_bytes(t) for t in tensors), index,
+            B, H, S, n, rows, first_ptr, first0, 1 if out is None else 0, stream,
+        )
+    nat.check(rc, "kvq_move_rows")
+
+
+def move_rows_paged(pools, pt: PageTable, index: torch.Tensor, *, first=0) -> None:
+    """move_rows in place over a paged cache's pools [H, rows, w]: position
+    index[b, h, i] of sequence b becomes its position first + i, through the
+    block table. A position whose page has no block moves nothing. Sequences
+    must not share the blocks that are written."""
+    what = "move_rows_paged"
+    pools = tuple(pools)
+    if not 1 <= len(pools) <= 5:
+        raise ValueError(f"{what}: 1 to 5 pools")
+    _check_cuda(*pools, index, pt.table, what=what)
+    H, rows = pools[0].shape[0], pt.num_blocks * pt.page_size
+    for p in pools:
+        if p.dim() != 3 or p.shape[:2] != (H, rows) or p.stride(2) != 1:
+            raise ValueError(f"{what}: pools must be [H={H}, num_blocks*page_size={rows}, w] with contiguous rows "
+                             f"(got {tuple(p.shape)})")
+        if p.device != pt.table.device:
+            raise ValueError(f"{what}: every tensor must be on one device")
+    if index.dim() != 3:
+        raise ValueError(f"{what}: index must be int32 [B, H or 1, n]")
+    B = index.shape[0]
+    if pt.table.shape[0] < B:
+        raise ValueError("block table has fewer rows than the batch")
+    index = _check_index(what, index, B, H, pools[0].device)
+    first_ptr, first0, first = _first(what, first, B, pools[0].device)
+    n = index.shape[2]
+    if B == 0 or H == 0 or n == 0 or any(p.shape[2] == 0 for p in pools):
+        return
+    with nat.device_of(index) as stream:
+        rc = nat.host().move_rows_paged(
+            pools, tuple(p.element_size() for p in pools), tuple(p.element_size() * p.shape[2] for p in pools),
+            pt.args(), index, B, H, n, first_ptr, first0, stream,
+        )
+    nat.check(rc, "kvq_move_rows_paged")
