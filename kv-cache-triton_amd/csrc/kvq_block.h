@@ -32,7 +32,7 @@ struct BlockArgs {
   void* out;
   int64_t os_b, os_h, os_s, os_d;
   // [B, Hq, T] (m, 1 / l) of each row, weight j = 2^(s_j - m) / l, or null. A row
-  // with no key, or no finite m, has 1 / l = 0. The pair, not m + log2 l: at
+  // with no key has 1 / l = 0. The pair, not m + log2 l: at
   // scores in the thousands the sum's rounding alone is 2^-12 of a weight.
   float2* stats;
   const int32_t* seq_lens;
@@ -53,6 +53,13 @@ __device__ __forceinline__ int64_t block_len(const BlockArgs& a, int b) {
 __device__ __forceinline__ bool block_sees(const BlockArgs& a, int b, int i, int64_t t) {
   if (a.kind == kMaskTree) return a.mask[b * a.ms_b + i * a.ms_i + t * a.ms_t] != 0;
   return a.kind == kMaskNone || t <= i;
+}
+
+// A score as the softmax takes it: NaN weighs nothing, and infinities are held
+// at finite values far outside any other score, so that no difference of two
+// scores is NaN.
+__device__ __forceinline__ float block_score(float s) {
+  return s == s ? fminf(fmaxf(s, -1.0e30f), 1.0e30f) : -__builtin_inff();
 }
 
 // Element d of a packed row: code - 8, exact in fp32.

@@ -1,0 +1,55 @@
+// The matrix-core kernel of kvq_block.hip: its arguments, plan and launch.
+#pragma once
+
+#include "kvq_block.h"
+
+namespace kvq {
+
+struct BlockMfmaArgs {
+  BlockArgs b;
+  int n_units, row_chunks, n_split;  // unit = batch * Hkv + KV head
+  int ng, s_f16;                     // scales of a cache row; whether they are fp16
+  int q_vec, o_vec;                  // 16-byte query pieces, 8-byte output pieces
+  int tiles_max;
+  float2* ws_ml;  // [unit][row][split] (max, sum)
+  float* ws_o;    // [unit][row][split][D] unnormalised
+  float* scores;  // [unit][tile][row][64], scores in log2 units, or null
+};
+
+struct BlockPlan {
+  int rb, nw;  // 16-row blocks a wave, waves a workgroup
+  int64_t row_chunks, n_split, ml_bytes, o_bytes;
+};
+
+BlockPlan block_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk);
+
+// Whether the kernel takes these arguments (else launch_block_rows).
+bool block_mfma_takes(const BlockArgs& a);
+
+// Without workspace for the plan's split the launch does not split.
+int launch_block_mfma(const BlockArgs& b, BlockPlan p, void* workspace, int64_t workspace_bytes, hipStream_t st);
+
+// Dims d .. d + 3 of output row R (row R / ratio of the block, head R % ratio
+// of the group), and the row's statistics, from a row's max, sum and
+// unnormalised values.
+template <bool QF16>
+__device__ __forceinline__ void block_store_row(const BlockMfmaArgs& a, int b, int kvh, int R, int d, float m, float l,
+                                                float4 o) {
+  const int i = R / a.b.ratio, h = kvh * a.b.ratio + R % a.b.ratio;
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  if (a.b.stats && d == 0) a.b.stats[((int64_t)b * a.b.Hq + h) * a.b.T + i] = make_float2(m, inv);
+  if (!a.b.out) return;
+  uint16_t* p = (uint16_t*)a.b.out + b * a.b.os_b + (int64_t)h * a.b.os_h + (int64_t)i * a.b.os_s + d;
+  const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = QF16 ? f32_to_f16_bits(v[k]) : f32_to_bf16_bits(v[k]);
+  if (a.o_vec) {
+    *(uint2*)p = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) p[k] = (uint16_t)w[k];
+  }
+}
+
+}  // namespace kvq

@@ -9,7 +9,7 @@
 // key is zero. The reference has no counterpart (its kernel masks causally,
 // kernels/llama3/attention_quant.py:91-97).
 
-#include "kvq_block.h"
+#include "kvq_block_mfma.h"
 
 namespace kvq {
 
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kRowThreads) void block_rows_kernel(const BlockArgs
         for (int e = 0; e < a.G && x < a.D; ++e, ++x) part_dot = fmaf(q_lds[x], code_at(kp + r * a.kps_s, x, a.G), part_dot);
         dot = fmaf(part_dot, load_as_f32(a.ks, ks0 + r * a.kss_s + g, a.s_dt), dot);
       }
-      s = dot == dot ? dot : -__builtin_inff();  // a NaN score weighs nothing
+      s = block_score(dot);
     }
     float mx = wave_max(s);
     if ((tid & 63) == 0) red[wave] = mx;
@@ -147,8 +147,7 @@ __global__ __launch_bounds__(kRowThreads) void block_rows_kernel(const BlockArgs
     for (int w = 0; w < kRowThreads / 64; ++w) mx = fmaxf(mx, red[w]);
     const float m_new = fmaxf(m, mx);
     const float alpha = m == m_new ? 1.0f : exp2f(m - m_new);
-    // (a score of +infinity takes all the weight)
-    const float p = s == -__builtin_inff() ? 0.0f : (s == m_new ? 1.0f : exp2f(s - m_new));
+    const float p = s == -__builtin_inff() ? 0.0f : exp2f(s - m_new);
     m = m_new;
     p_lds[tid] = p;
     row_lds[tid] = r;
@@ -173,7 +172,7 @@ __global__ __launch_bounds__(kRowThreads) void block_rows_kernel(const BlockArgs
 #pragma unroll
   for (int w = 0; w < kRowThreads / 64; ++w) l += red[w];
   if (a.stats && tid == 0)
-    a.stats[((int64_t)b * a.Hq + h) * a.T + i] = make_float2(m, l > 0.0f && m < __builtin_inff() ? 1.0f / l : 0.0f);
+    a.stats[((int64_t)b * a.Hq + h) * a.T + i] = make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
   if (a.out && tid < a.D) {
     float x = 0.0f;
     for (int w = 0; w < parts; ++w) x += o_lds[w * a.D + tid];
@@ -214,9 +213,12 @@ int tree_impl(const char* what, const void* q, int q_dtype, const int64_t* q_str
   a.ms_b = mask_strides[0]; a.ms_i = mask_strides[1]; a.ms_t = mask_strides[2];
   a.out = out;
   a.os_b = out_strides[0]; a.os_h = out_strides[1]; a.os_s = out_strides[2]; a.os_d = out_strides[3];
-  (void)workspace;
-  (void)workspace_bytes;
-  launch_block_rows(a, (hipStream_t)stream);
+  if (block_mfma_takes(a)) {
+    const int lc = launch_block_mfma(a, block_plan(B, Hq, Hkv, T, D, Sk), workspace, workspace_bytes, (hipStream_t)stream);
+    KVQ_CHECK_ARG(lc == KVQ_OK, "%s: too large", what);
+  } else {
+    launch_block_rows(a, (hipStream_t)stream);
+  }
   KVQ_CHECK_LAUNCH(what);
   return KVQ_OK;
 }
@@ -258,5 +260,7 @@ extern "C" int64_t kvq_tree_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t 
     set_error("kvq_tree_attn_workspace_bytes: bad shape or dtype");
     return KVQ_EINVAL;
   }
-  return 0;
+  if (B == 0 || T == 0 || !(D == 64 || D == 128) || q_dtype == KVQ_F32 || scale_dtype == KVQ_F32) return 0;
+  const BlockPlan p = block_plan(B, Hq, Hkv, T, D, Sk);
+  return p.ml_bytes + p.o_bytes;
 }

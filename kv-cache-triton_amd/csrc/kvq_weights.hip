@@ -54,8 +54,7 @@ __global__ __launch_bounds__(kWThreads) void key_weights_rows_kernel(const Block
         dot = fmaf(load_as_f32(a.q, q0 + d * a.qs_d, a.q_dt) * a.scale_log2, k_lds[key * pitch + d], dot);
       s = fmaf(dot, load_as_f32(a.ks, ks0 + j * a.kss_s + g, a.s_dt), s);
     }
-    const float p = exp2f(s - st.x) * st.y;
-    sum += p == p ? p : 0.0f;  // (a NaN score weighs nothing)
+    sum = fmaf(exp2f(block_score(s) - st.x), st.y, sum);
   }
   sums[tid] = sum;
   __syncthreads();
