@@ -121,16 +121,24 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const f16x2_t h = {(_Float16)lo, (_Float16)hi};
   return __builtin_bit_cast(uint32_t, h);
 }
+// (x & m) | o in one instruction: with constants in plain sight the compiler
+// writes two, each with its literal.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
+  uint32_t d;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(d) : "v"(x), "s"(m), "v"(o));
+  return d;
+}
+
 // The eight nibbles of w as 16-bit floats 16 + n: pair p is (nibble p, nibble
 // p + 4). The queries are put in the same order.
 template <bool F16>
 __device__ __forceinline__ uint4 unpack_keys(uint32_t w) {
   if constexpr (F16) {
     constexpr uint32_t m = 0x03c003c0u, o = 0x4c004c00u;
-    return make_uint4(((w << 6) & m) | o, ((w << 2) & m) | o, ((w >> 2) & m) | o, ((w >> 6) & m) | o);
+    return make_uint4(and_or(w << 6, m, o), and_or(w << 2, m, o), and_or(w >> 2, m, o), and_or(w >> 6, m, o));
   } else {
     constexpr uint32_t m = 0x00780078u, o = 0x41804180u;
-    return make_uint4(((w << 3) & m) | o, ((w >> 1) & m) | o, ((w >> 5) & m) | o, ((w >> 9) & m) | o);
+    return make_uint4(and_or(w << 3, m, o), and_or(w >> 1, m, o), and_or(w >> 5, m, o), and_or(w >> 9, m, o));
   }
 }
 __device__ __forceinline__ uint4 pair_queries(uint4 x) {  // dims (0, 4), (1, 5), (2, 6), (3, 7)
@@ -141,14 +149,14 @@ __device__ __forceinline__ uint4 pair_queries(uint4 x) {  // dims (0, 4), (1, 5)
 // A pair of codes (4-bit fields `shift` of y's halves) as fp16 n - 8, times a
 // pair of scales.
 __device__ __forceinline__ uint32_t value_pair(uint32_t y, int shift, uint32_t scales) {
-  const uint32_t x = ((y >> shift) & 0x000f000fu) | 0x64006400u;
+  const uint32_t x = and_or(y >> shift, 0x000f000fu, 0x64006400u);
   const f16x2_t off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
   const f16x2_t v = (__builtin_bit_cast(f16x2_t, x) + off) * __builtin_bit_cast(f16x2_t, scales);
   return __builtin_bit_cast(uint32_t, v);
 }
 
 template <int D, bool QF16, int RB, int NW, bool PAGED, bool SCORES>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RB == 4 ? 1 : 2)))
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
 void block_attn_kernel(const BlockMfmaArgs a) {
   constexpr int NC = D / 32;    // 32-dim chunks
   constexpr int VN = D / 16;    // 16-dim blocks of O^T; dims a lane holds of a value row
@@ -647,8 +655,7 @@ void launch_block(const BlockMfmaArgs& a, hipStream_t st) {
 template <int D, bool QF16>
 void launch_rb(const BlockMfmaArgs& a, int rb, hipStream_t st) {
   if (rb == 1) launch_block<D, QF16, 1, 8, false>(a, st);
-  else if (rb == 2) launch_block<D, QF16, 2, 8, false>(a, st);
-  else launch_block<D, QF16, 4, 4, false>(a, st);
+  else launch_block<D, QF16, 2, 8, false>(a, st);
 }
 
 }  // namespace
@@ -656,12 +663,24 @@ void launch_rb(const BlockMfmaArgs& a, int rb, hipStream_t st) {
 BlockPlan block_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk) {
   const int64_t rows = T * (Hq / Hkv), units = B * Hkv;
   BlockPlan p;
-  p.rb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  p.nw = p.rb == 4 ? 4 : 8;
+  p.rb = rows <= 16 ? 1 : 2;
+  p.nw = 8;
   p.row_chunks = (rows + 16 * p.rb - 1) / (16 * p.rb);
+  // the split with the least estimate: rounds of one workgroup per CU, each its
+  // waves' tiles and about two tiles' time of prologue and epilogue; a merge
+  // costs about a tile's time and its partials' traffic
   const int64_t tiles = (Sk + kKeys - 1) / kKeys, wgs = units * p.row_chunks;
   p.n_split = 1;
-  if (wgs > 0) p.n_split = std::max<int64_t>(1, std::min<int64_t>((256 + wgs - 1) / wgs, (tiles + p.nw - 1) / p.nw));
+  double best = 0.0;
+  for (int64_t ns = 1; ns <= std::min<int64_t>(64, std::max<int64_t>(1, (tiles + p.nw - 1) / p.nw)); ++ns) {
+    const double rounds = (double)((wgs * ns + 255) / 256);
+    const double cost = rounds * ((double)((tiles + ns * p.nw - 1) / (ns * p.nw)) + 2.0) +
+                        (ns > 1 ? 1.0 + (double)(units * rows * ns) * (double)D * 8.0 / 8.0e6 : 0.0);
+    if (ns == 1 || cost < best) {
+      best = cost;
+      p.n_split = ns;
+    }
+  }
   p.ml_bytes = 0;
   p.o_bytes = 0;
   if (p.n_split > 1) {
