@@ -430,12 +430,13 @@ void block_attn_kernel(const BlockMfmaArgs a) {
     if constexpr (SCORES) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        float* dst = a.scores + (((int64_t)unit * a.tiles_max + t) * (a.row_chunks * ROWS) + chunk * ROWS + 16 * r + n) * kKeys;
+        float* dst = a.scores + (((int64_t)unit * a.tiles_max + t) * rows + chunk * ROWS + 16 * r + n) * kKeys;
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[r][kb][j] *= c;
-          *(float4*)(dst + 16 * kb + 4 * g) = make_float4(s[r][kb][0], s[r][kb][1], s[r][kb][2], s[r][kb][3]);
+          if (row_i[r] >= 0)
+            *(float4*)(dst + 16 * kb + 4 * g) = make_float4(s[r][kb][0], s[r][kb][1], s[r][kb][2], s[r][kb][3]);
         }
       }
     }
@@ -583,27 +584,19 @@ void block_attn_kernel(const BlockMfmaArgs a) {
       }
       const int R = chunk * ROWS + 16 * r + row;
       if (R >= rows) continue;
-      if (a.n_split > 1) {
-        const int64_t slot = ((int64_t)unit * rows + R) * a.n_split + sp;
-        *(float4*)(a.ws_o + slot * D + d) = acc;
-        if (d == 0) a.ws_ml[slot] = make_float2(Mr, L);
-      } else {
-        block_store_row<QF16>(a, b, kvh, R, d, Mr, L, acc);
-      }
+      const int64_t slot = ((int64_t)unit * rows + R) * a.n_split + sp;
+      if ((SCORES || a.n_split > 1) && d == 0) a.ws_ml[slot] = make_float2(Mr, L);
+      if (a.n_split > 1) *(float4*)(a.ws_o + slot * D + d) = acc;
+      else block_store_row<QF16>(a, b, kvh, R, d, Mr, L, acc);
     }
     if (r + 1 < RB) __syncthreads();
   }
 }
 
-// Combines the splits' partials of a row (log-sum-exp in base 2): a thread owns
-// four dims. Memory-bound: it reads every partial once.
+// Combines the splits' partials of row `row` (log-sum-exp in base 2) in dims
+// d .. d + 3 and stores them. Memory-bound: it reads every partial once.
 template <int D, bool QF16>
-__global__ __launch_bounds__(256) void block_merge_kernel(const BlockMfmaArgs a) {
-  constexpr int RPW = 1024 / D;
-  const int rows = a.b.ratio * a.b.T;
-  const int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / (D / 4);
-  if (row >= (int64_t)a.n_units * rows) return;
-  const int d = 4 * (threadIdx.x % (D / 4));
+__device__ __forceinline__ void merge_row(const BlockMfmaArgs& a, int64_t row, int rows, int d) {
   const int unit = (int)(row / rows), R = (int)(row % rows);
   const int64_t slot = row * a.n_split;
   float M = kNeg, L = 0.0f;
@@ -637,6 +630,59 @@ __global__ __launch_bounds__(256) void block_merge_kernel(const BlockMfmaArgs a)
   block_store_row<QF16>(a, unit / a.b.Hkv, unit % a.b.Hkv, R, d, M, L, acc);
 }
 
+template <int D, bool QF16>
+__global__ __launch_bounds__(256) void block_merge_kernel(const BlockMfmaArgs a) {
+  const int rows = a.b.ratio * a.b.T;
+  const int64_t row = (int64_t)blockIdx.x * (1024 / D) + threadIdx.x / (D / 4);
+  if (row < (int64_t)a.n_units * rows) merge_row<D, QF16>(a, row, rows, 4 * (threadIdx.x % (D / 4)));
+}
+
+// After a launch that kept its scores: each key's weights from them and the
+// rows' statistics, and (in workgroups of their own) the splits' merge. A
+// thread owns one key; scores are read in their storage order. Memory-bound:
+// rows * 4 bytes a key, and the running sum once.
+constexpr int kFinishKeys = 256;
+
+template <int D, bool QF16>
+__global__ __launch_bounds__(256) void block_finish_kernel(const BlockMfmaArgs a, int key_wgs) {
+  __shared__ float2 st[kMaxScoreRows];
+  const int rows = a.b.ratio * a.b.T;
+  if ((int)blockIdx.x >= key_wgs) {
+    const int64_t row = (int64_t)(blockIdx.x - key_wgs) * (1024 / D) + threadIdx.x / (D / 4);
+    if (row < (int64_t)a.n_units * rows) merge_row<D, QF16>(a, row, rows, 4 * (threadIdx.x % (D / 4)));
+    return;
+  }
+  const int unit = blockIdx.x % a.n_units, tile0 = (blockIdx.x / a.n_units) * (kFinishKeys / kKeys);
+  const int kvh = unit % a.b.Hkv, b = unit / a.b.Hkv;
+  const int len = (int)block_len(a.b, b);
+  if (tile0 * kKeys >= len) return;
+  if ((int)threadIdx.x < rows) {
+    const float2* ml = a.ws_ml + ((int64_t)unit * rows + threadIdx.x) * a.n_split;
+    float M = kNeg, L = 0.0f;
+    for (int s = 0; s < a.n_split; ++s) M = fmaxf(M, ml[s].x);
+    for (int s = 0; s < a.n_split; ++s) L = fmaf(ml[s].y, __builtin_amdgcn_exp2f(ml[s].x - M), L);
+    st[threadIdx.x] = make_float2(M, L > 0.0f ? 1.0f / L : 0.0f);
+  }
+  __syncthreads();
+  const int tile = tile0 + threadIdx.x / kKeys, pos = threadIdx.x % kKeys;
+  const int key = tile * kKeys + (pos & 48) + ((pos >> 2) & 3) + 4 * (pos & 3);
+  if (tile * kKeys >= len) return;
+  const float* sc = a.scores + ((int64_t)unit * a.tiles_max + tile) * rows * kKeys + pos;
+  float* w = a.weights + b * a.w_b + kvh * a.w_h + key * a.w_k;
+  const bool on = key < len;
+  const float before = on ? *w : 0.0f;
+  float sum = 0.0f;
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = sc[min(r0 + k, rows - 1) * kKeys];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (r0 + k < rows) sum = fmaf(__builtin_amdgcn_exp2f(x[k] - st[r0 + k].x), st[r0 + k].y, sum);
+  }
+  if (on) *w = before + sum;
+}
+
 template <int D, bool QF16, int RB, int NW, bool SCORES>
 void launch_block(const BlockMfmaArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.n_units * a.row_chunks * a.n_split)), block(64 * NW);
@@ -654,6 +700,17 @@ void launch_block(const BlockMfmaArgs& a, hipStream_t st) {
 
 template <int D, bool QF16>
 void launch_rb(const BlockMfmaArgs& a, int rb, hipStream_t st) {
+  if (a.scores) {
+    if (rb == 1) launch_block<D, QF16, 1, 8, true>(a, st);
+    else launch_block<D, QF16, 2, 8, true>(a, st);
+    const int key_wgs = a.n_units * ((a.tiles_max * kKeys + kFinishKeys - 1) / kFinishKeys);
+    const int64_t rows = (int64_t)a.n_units * a.b.ratio * a.b.T;
+    const int merge_wgs = a.n_split > 1 ? (int)((rows + 1024 / D - 1) / (1024 / D)) : 0;
+    if (key_wgs + merge_wgs > 0)
+      hipLaunchKernelGGL((block_finish_kernel<D, QF16>), dim3((unsigned)(key_wgs + merge_wgs)), dim3(256), 0, st, a,
+                         key_wgs);
+    return;
+  }
   if (rb == 1) launch_block<D, QF16, 1, 8, false>(a, st);
   else launch_block<D, QF16, 2, 8, false>(a, st);
 }
@@ -690,38 +747,47 @@ BlockPlan block_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, i
   return p;
 }
 
-bool block_mfma_takes(const BlockArgs& a) {
+namespace {
+bool dense_rows(const void* p, int64_t b, int64_t h, int64_t s, int64_t row, int64_t n, int64_t size) {
+  return s == row && (uintptr_t)p % (n * size) == 0 && b % n == 0 && h % n == 0;
+}
+}  // namespace
+
+bool block_mfma_takes_keys(const BlockArgs& a) {
   if (!(a.D == 64 || a.D == 128) || !(a.G == 32 || a.G == 64 || a.G == 128) || a.D % a.G != 0) return false;
-  const int ng = a.D / a.G, kb = a.D / 8;  // scales of a row, bytes of a key load
-  auto rows = [](const void* p, int64_t b, int64_t h, int64_t s, int64_t row, int64_t n, int64_t size) {
-    return s == row && (uintptr_t)p % (n * size) == 0 && b % n == 0 && h % n == 0;
-  };
-  return a.q_dt != KVQ_F32 && a.s_dt != KVQ_F32 && a.qs_d == 1 && a.os_d == 1 &&
-         (!a.pm.paged || (a.pm.page_shift >= 6 && a.pm.n_pages > 0)) && a.Sk < (int64_t(1) << 30) &&
-         rows(a.kp, a.kps_b, a.kps_h, a.kps_s, a.D / 2, kb, 1) && rows(a.vp, a.vps_b, a.vps_h, a.vps_s, a.D / 2, 4, 1) &&
-         rows(a.ks, a.kss_b, a.kss_h, a.kss_s, ng, ng, 2) && rows(a.vs, a.vss_b, a.vss_h, a.vss_s, ng, ng, 2);
+  const int ng = a.D / a.G;
+  return a.q_dt != KVQ_F32 && a.s_dt != KVQ_F32 && a.qs_d == 1 && (!a.pm.paged || (a.pm.page_shift >= 6 && a.pm.n_pages > 0)) &&
+         a.Sk < (int64_t(1) << 30) && dense_rows(a.kp, a.kps_b, a.kps_h, a.kps_s, a.D / 2, a.D / 8, 1) &&
+         dense_rows(a.ks, a.kss_b, a.kss_h, a.kss_s, ng, ng, 2);
 }
 
-int launch_block_mfma(const BlockArgs& b, BlockPlan p, void* workspace, int64_t workspace_bytes, hipStream_t st) {
-  if (p.n_split > 1 && (workspace == nullptr || workspace_bytes < p.ml_bytes + p.o_bytes || (uintptr_t)workspace % 16 != 0))
-    p.n_split = 1;
-  BlockMfmaArgs a = {};
-  a.b = b;
-  a.n_units = b.B * b.Hkv;
-  a.row_chunks = (int)p.row_chunks;
-  a.n_split = (int)p.n_split;
-  a.ng = b.D / b.G;
-  a.s_f16 = b.s_dt == KVQ_F16;
-  a.ws_ml = (float2*)workspace;
-  a.ws_o = (float*)((char*)workspace + p.ml_bytes);
+bool block_mfma_takes(const BlockArgs& a) {
+  return block_mfma_takes_keys(a) && a.os_d == 1 && dense_rows(a.vp, a.vps_b, a.vps_h, a.vps_s, a.D / 2, 4, 1) &&
+         dense_rows(a.vs, a.vss_b, a.vss_h, a.vss_s, a.D / a.G, a.D / a.G, 2);
+}
+
+namespace {
+
+void fill_mfma(BlockMfmaArgs* a, const BlockArgs& b, const BlockPlan& p) {
+  *a = BlockMfmaArgs{};
+  a->b = b;
+  a->n_units = b.B * b.Hkv;
+  a->row_chunks = (int)p.row_chunks;
+  a->n_split = (int)p.n_split;
+  a->ng = b.D / b.G;
+  a->s_f16 = b.s_dt == KVQ_F16;
+  a->tiles_max = (int)((b.Sk + kKeys - 1) / kKeys);
   auto mult = [](const void* p, int64_t bytes, int64_t s0, int64_t s1, int64_t s2, int64_t n) {
     return (uintptr_t)p % bytes == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0;
   };
-  a.q_vec = mult(b.q, 16, b.qs_b, b.qs_h, b.qs_s, 8);
-  a.o_vec = b.out && mult(b.out, 8, b.os_b, b.os_h, b.os_s, 4);
+  a->q_vec = mult(b.q, 16, b.qs_b, b.qs_h, b.qs_s, 8);
+  a->o_vec = b.out && mult(b.out, 8, b.os_b, b.os_h, b.os_s, 4);
+}
+
+int launch_any(const BlockMfmaArgs& a, const BlockPlan& p, hipStream_t st) {
   if ((int64_t)a.n_units * a.row_chunks * a.n_split >= (int64_t(1) << 31)) return KVQ_EUNSUP;
-  const bool f16 = b.q_dt == KVQ_F16;
-  if (b.D == 128) {
+  const bool f16 = a.b.q_dt == KVQ_F16;
+  if (a.b.D == 128) {
     if (f16) launch_rb<128, true>(a, p.rb, st);
     else launch_rb<128, false>(a, p.rb, st);
   } else {
@@ -729,6 +795,41 @@ int launch_block_mfma(const BlockArgs& b, BlockPlan p, void* workspace, int64_t 
     else launch_rb<64, false>(a, p.rb, st);
   }
   return KVQ_OK;
+}
+
+}  // namespace
+
+int launch_block_mfma(const BlockArgs& b, BlockPlan p, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+  if (p.n_split > 1 && (workspace == nullptr || workspace_bytes < p.ml_bytes + p.o_bytes || (uintptr_t)workspace % 16 != 0))
+    p.n_split = 1;
+  BlockMfmaArgs a;
+  fill_mfma(&a, b, p);
+  a.ws_ml = (float2*)workspace;
+  a.ws_o = (float*)((char*)workspace + p.ml_bytes);
+  return launch_any(a, p, st);
+}
+
+int64_t block_scores_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk) {
+  const int64_t rows = T * (Hq / Hkv);
+  if (rows > kMaxScoreRows) return 0;
+  const BlockPlan p = block_plan(B, Hq, Hkv, T, D, Sk);
+  const int64_t ml = (B * Hkv * rows * p.n_split * 8 + 255) / 256 * 256;
+  return ml + p.o_bytes + B * Hkv * ((Sk + kKeys - 1) / kKeys) * rows * kKeys * 4;
+}
+
+int launch_block_weights(const BlockArgs& b, float* weights, const int64_t* ws, void* workspace, hipStream_t st) {
+  const int64_t rows = (int64_t)b.ratio * b.T;
+  const BlockPlan p = block_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk);
+  BlockMfmaArgs a;
+  fill_mfma(&a, b, p);
+  const int64_t ml = ((int64_t)a.n_units * rows * p.n_split * 8 + 255) / 256 * 256;
+  a.ws_ml = (float2*)workspace;
+  a.ws_o = (float*)((char*)workspace + ml);
+  a.scores = (float*)((char*)workspace + ml + p.o_bytes);
+  a.weights = weights;
+  a.w_b = ws[0]; a.w_h = ws[1]; a.w_k = ws[2];
+  if ((int64_t)a.n_units * (a.tiles_max / 4 + 1) + a.n_units * rows >= (int64_t(1) << 31)) return KVQ_EUNSUP;
+  return launch_any(a, p, st);
 }
 
 }  // namespace kvq

@@ -13,8 +13,14 @@ struct BlockMfmaArgs {
   int tiles_max;
   float2* ws_ml;  // [unit][row][split] (max, sum)
   float* ws_o;    // [unit][row][split][D] unnormalised
-  float* scores;  // [unit][tile][row][64], scores in log2 units, or null
+  // key weights: scores in log2 units ([unit][tile][row][64], the keys of a
+  // tile in the order 16 kb + g + 4 j at 16 kb + 4 g + j), or null, and the sums
+  float* scores;
+  float* weights;
+  int64_t w_b, w_h, w_k;
 };
+
+constexpr int kMaxScoreRows = 32;  // query rows per KV head of a launch that keeps its scores
 
 struct BlockPlan {
   int rb, nw;  // 16-row blocks a wave, waves a workgroup
@@ -23,11 +29,18 @@ struct BlockPlan {
 
 BlockPlan block_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk);
 
-// Whether the kernel takes these arguments (else launch_block_rows).
+// Whether the matrix-core kernels take these arguments (else the plain ones);
+// the first for kernels that read no values.
+bool block_mfma_takes_keys(const BlockArgs& a);
 bool block_mfma_takes(const BlockArgs& a);
 
 // Without workspace for the plan's split the launch does not split.
 int launch_block_mfma(const BlockArgs& b, BlockPlan p, void* workspace, int64_t workspace_bytes, hipStream_t st);
+
+// Attention that keeps its scores, and the key weights from them, for up to
+// kMaxScoreRows rows per KV head; workspace bytes (0 for more rows).
+int64_t block_scores_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk);
+int launch_block_weights(const BlockArgs& b, float* weights, const int64_t* ws, void* workspace, hipStream_t st);
 
 // Dims d .. d + 3 of output row R (row R / ratio of the block, head R % ratio
 // of the group), and the row's statistics, from a row's max, sum and

@@ -11,7 +11,9 @@
 // ranks the cache's rows by. Sums over rows are taken in a fixed order (no
 // atomics), so equal calls give equal bits. The reference has no counterpart.
 
-#include "kvq_block.h"
+#include <algorithm>
+
+#include "kvq_block_mfma.h"
 
 namespace kvq {
 namespace {
@@ -73,6 +75,22 @@ void launch_key_weights_rows(const BlockArgs& a, float* w, const int64_t* ws, hi
 
 int64_t stats_bytes(int64_t B, int64_t Hq, int64_t T) { return (B * Hq * T * 8 + 255) / 256 * 256; }
 
+// Whether a call with attention keeps its scores (launch_block_weights): few
+// rows per KV head, as of decode tokens, and scores of at most 1 GiB.
+bool takes_scores(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, int q_dt, int s_dt) {
+  if (!(D == 64 || D == 128) || q_dt == KVQ_F32 || s_dt == KVQ_F32) return false;
+  const int64_t n = block_scores_bytes(B, Hq, Hkv, T, D, Sk);
+  return n > 0 && n <= (int64_t(1) << 30);
+}
+
+int64_t workspace_needed(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, int q_dt, int s_dt,
+                         bool with_out) {
+  int64_t n = stats_bytes(B, Hq, T);
+  if (B > 0 && T > 0 && with_out && takes_scores(B, Hq, Hkv, T, D, Sk, q_dt, s_dt))
+    n = std::max(n, block_scores_bytes(B, Hq, Hkv, T, D, Sk));
+  return n;
+}
+
 // Shared by the two entry points: with `out`, the block's attention too.
 int weights_impl(const char* what, const void* q, int q_dtype, const int64_t* q_strides, const void* k_packed,
                  const int64_t* kp_strides, const void* k_scales, const int64_t* ks_strides, const void* v_packed,
@@ -90,8 +108,9 @@ int weights_impl(const char* what, const void* q, int q_dtype, const int64_t* q_
   if (B == 0 || T == 0) return KVQ_OK;
   KVQ_CHECK_ARG(B * Hkv * ((Sk + kWKeys - 1) / kWKeys) < (int64_t(1) << 31), "%s: too large", what);
   KVQ_CHECK_ARG(q && (!vp_strides || out) && (weights || Sk == 0), "%s: null data pointer", what);
-  if (workspace == nullptr || workspace_bytes < stats_bytes(B, Hq, T) || (uintptr_t)workspace % 16 != 0) {
-    set_error("%s: a 16-byte aligned workspace of %lld bytes is needed", what, (long long)stats_bytes(B, Hq, T));
+  const int64_t need = workspace_needed(B, Hq, Hkv, T, D, Sk, q_dtype, scale_dtype, vp_strides != nullptr);
+  if (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0) {
+    set_error("%s: a 16-byte aligned workspace of %lld bytes is needed", what, (long long)need);
     return KVQ_ESPACE;
   }
   a.kind = is_causal ? kMaskCausal : kMaskNone;
@@ -101,6 +120,13 @@ int weights_impl(const char* what, const void* q, int q_dtype, const int64_t* q_
     a.os_b = out_strides[0]; a.os_h = out_strides[1]; a.os_s = out_strides[2]; a.os_d = out_strides[3];
   }
   hipStream_t st = (hipStream_t)stream;
+  if (a.out && takes_scores(B, Hq, Hkv, T, D, Sk, q_dtype, scale_dtype) && block_mfma_takes(a)) {
+    a.stats = nullptr;
+    const int lc = launch_block_weights(a, weights, weight_strides, workspace, st);
+    KVQ_CHECK_ARG(lc == KVQ_OK, "%s: too large", what);
+    KVQ_CHECK_LAUNCH(what);
+    return KVQ_OK;
+  }
   launch_block_rows(a, st);
   launch_key_weights_rows(a, weights, weight_strides, st);
   KVQ_CHECK_LAUNCH(what);
@@ -148,6 +174,5 @@ extern "C" int64_t kvq_key_weights_workspace_bytes(int64_t B, int64_t Hq, int64_
     set_error("kvq_key_weights_workspace_bytes: bad shape or dtype");
     return KVQ_EINVAL;
   }
-  (void)with_attention;
-  return stats_bytes(B, Hq, Sq);
+  return workspace_needed(B, Hq, Hkv, Sq, D, Sk, q_dtype, scale_dtype, with_attention != 0);
 }
