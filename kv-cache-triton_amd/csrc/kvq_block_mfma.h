@@ -42,6 +42,11 @@ int launch_block_mfma(const BlockArgs& b, BlockPlan p, void* workspace, int64_t 
 int64_t block_scores_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk);
 int launch_block_weights(const BlockArgs& b, float* weights, const int64_t* ws, void* workspace, hipStream_t st);
 
+// Key weights of blocks of any length (kvq_sums.hip), for what
+// block_mfma_takes_keys takes of a contiguous cache.
+int64_t sums_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t Sk, bool s_f16);
+int launch_key_sums(const BlockArgs& b, float* weights, const int64_t* ws, void* workspace, hipStream_t st);
+
 // Dims d .. d + 3 of output row R (row R / ratio of the block, head R % ratio
 // of the group), and the row's statistics, from a row's max, sum and
 // unnormalised values.

@@ -1251,6 +1251,17 @@ def attention_with_key_weights(
     _check_cache(what, q, (k_packed, k_scales, v_packed, v_scales), B, n_kv_heads, D, group_size)
     Sk = k_packed.shape[2]
     _check_weights(what, key_weights, B, n_kv_heads, Sk)
+    if seq_lens is None and use_prefill_kernel(Hq // n_kv_heads * Sq, Sk):
+        # long blocks: the prefill kernels, and the weights beside them
+        try:
+            prefill_attention(q, k_packed, k_scales, v_packed, v_scales, n_kv_heads=n_kv_heads, group_size=group_size,
+                              is_causal=is_causal, sm_scale=sm_scale, out=out)
+        except nat.KVQUnsupported:
+            pass
+        else:
+            add_key_weights(q, k_packed, k_scales, key_weights, n_kv_heads=n_kv_heads, group_size=group_size,
+                            is_causal=is_causal, sm_scale=sm_scale)
+            return out
     sl_ptr, seq_lens = _lens_ptr(what, seq_lens, B, q.device)
     qd, sd = nat.DTYPE_CODE[q.dtype], nat.DTYPE_CODE[k_scales.dtype]
     with nat.device_of(q) as stream:
