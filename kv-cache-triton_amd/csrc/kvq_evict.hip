@@ -39,63 +39,168 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
 
 __device__ __forceinline__ int wave_count(bool x) { return __builtin_popcountll(__builtin_amdgcn_ballot_w64(x)); }
 
-// One workgroup per (sequence, KV head). The rank of the k-th largest weight
-// is built bit by bit from the top (32 counts over the candidates), then one
-// ordered pass writes the rows above it and the first of those that equal it.
+struct SelectUnit {
+  const float* w;
+  int32_t* out;
+  int n, lo, hi, want;  // candidates [lo, hi), of which `want` are kept
+};
+
+__device__ __forceinline__ SelectUnit select_unit(const SelectArgs& a) {
+  const int h = blockIdx.x % a.H, b = blockIdx.x / a.H;
+  int64_t n = a.S;
+  if (a.seq_lens) {
+    n = a.seq_lens[b];
+    n = n < 0 ? 0 : (n > a.S ? a.S : n);
+  }
+  SelectUnit u;
+  u.w = a.w + b * a.ws_b + h * a.ws_h;
+  u.out = a.index + ((int64_t)b * a.H + h) * a.keep;
+  u.n = (int)n;
+  u.lo = a.sink;
+  u.hi = u.n - a.recent;
+  u.want = a.keep - a.sink - a.recent;
+  return u;
+}
+
+// A sequence that keeps everything.
+__device__ __forceinline__ void select_all(const SelectArgs& a, const SelectUnit& u) {
+  for (int i = threadIdx.x; i < a.keep; i += kSelThreads) u.out[i] = i < u.n ? i : -1;
+}
+
+// Sum over the workgroup's waves of a value uniform in each wave; `slot`
+// alternates between two calls' buffers, so that one barrier is enough.
+__device__ __forceinline__ int block_sum(int x, int* slot) {
+  if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kSelThreads / 64; ++w) total += slot[w];
+  return total;
+}
+
+// One workgroup per (sequence, KV head), its ranks in registers (NE a thread;
+// each wave holds 64 NE consecutive rows, so that its kept rows are counted
+// and written in order). The rank of the want-th largest is built bit by bit
+// from the top: a bit is set if that many candidates are at least the rank so
+// formed, counted with one compare a register and ballots (a histogram in LDS
+// would put most of a wave's lanes on the same few exponents). It stops as soon
+// as exactly `want` candidates are at or above it. Bound by those compares and a
+// barrier a bit, about 0.2 us a bit at 16K keys.
+template <int NE>
 __global__ __launch_bounds__(kSelThreads) void select_keys_kernel(const SelectArgs a) {
   __shared__ int counts[2][kSelThreads / 64];
-  __shared__ int above[kSelThreads / 64], equal[kSelThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int h = blockIdx.x % a.H, b = blockIdx.x / a.H;
-  int64_t n64 = a.S;
-  if (a.seq_lens) {
-    n64 = a.seq_lens[b];
-    n64 = n64 < 0 ? 0 : (n64 > a.S ? a.S : n64);
-  }
-  const int n = (int)n64;
-  const float* w = a.w + b * a.ws_b + h * a.ws_h;
-  int32_t* out = a.index + ((int64_t)b * a.H + h) * a.keep;
-  if (n <= a.keep) {
-    for (int i = tid; i < a.keep; i += kSelThreads) out[i] = i < n ? i : -1;
+  const SelectUnit u = select_unit(a);
+  if (u.n <= a.keep) {
+    select_all(a, u);
     return;
   }
-  const int lo = a.sink, hi = n - a.recent;  // candidates [lo, hi): keep > sink + recent or none is taken
-  const int want = a.keep - a.sink - a.recent;
-  uint32_t t = 0;  // the want-th largest rank
-  if (want > 0) {
-    for (int bit = 31; bit >= 0; --bit) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j0 = wave * (64 * NE) + lane;
+  uint32_t r[NE];  // ranks of rows j0 + 64 e; 0 (below every rank) outside the candidates
+#pragma unroll
+  for (int e = 0; e < NE; ++e) {
+    const int j = j0 + 64 * e;
+    r[e] = j >= u.lo && j < u.hi ? rank_of(u.w[(int64_t)j * a.ws_k]) : 0u;
+  }
+  uint32_t t = 0;
+  bool exact = u.want == 0;  // whether the candidates at or above t are just those kept
+  if (!exact) {
+#pragma unroll 1
+    for (int bit = 31; bit >= 0 && !exact; --bit) {
       const uint32_t cand = t | (1u << bit);
       int c = 0;
-      for (int j = lo + tid; j - tid < hi; j += kSelThreads)
-        c += wave_count(j < hi && rank_of(w[(int64_t)j * a.ws_k]) >= cand);
-      int* slot = counts[bit & 1];
-      if (lane == 0) slot[wave] = c;
-      __syncthreads();
-      int total = 0;
 #pragma unroll
-      for (int x = 0; x < kSelThreads / 64; ++x) total += slot[x];
-      if (total >= want) t = cand;
+      for (int e = 0; e < NE; ++e) c += wave_count(r[e] >= cand);
+      const int total = block_sum(c, counts[bit & 1]);
+      if (total >= u.want) {
+        t = cand;
+        exact = total == u.want;
+      }
     }
   } else {
     t = 0xffffffffu;
   }
-  // rows in order, 1024 at a time: [0, sink) and [hi, n) always, a candidate
-  // above t, and of those equal to t the first `ties`
-  int n_above = 0;
-  for (int j = lo + tid; j - tid < hi; j += kSelThreads)
-    n_above += wave_count(j < hi && want > 0 && rank_of(w[(int64_t)j * a.ws_k]) > t);
-  __syncthreads();
-  if (lane == 0) counts[0][wave] = n_above;
-  __syncthreads();
-  int ties = want;
+  // of the candidates that equal t, the first `ties` (exact: all of them)
+  int above = 0, equal = 0;
 #pragma unroll
-  for (int x = 0; x < kSelThreads / 64; ++x) ties -= counts[0][x];
+  for (int e = 0; e < NE; ++e) {
+    above += wave_count(r[e] > t);
+    equal += wave_count(r[e] == t && t != 0u);
+  }
+  if (u.want == 0) above = equal = 0;
+  __syncthreads();
+  const int all_above = block_sum(above, counts[0]);
+  int ties = u.want - all_above, before = 0;
+  (void)block_sum(equal, counts[1]);
+#pragma unroll
+  for (int w = 0; w < kSelThreads / 64; ++w) before += w < wave ? counts[1][w] : 0;
+  // rows kept in this wave, its place among the waves', then the rows again
+  auto keeps = [&](int e, int& seen) {  // the wave's kept rows among its e-th 64; seen: ties so far
+    const int j = j0 + 64 * e;
+    const bool cand = u.want > 0 && j >= u.lo && j < u.hi;
+    const bool tie = cand && r[e] == t;
+    const uint64_t mt = __builtin_amdgcn_ballot_w64(tie);
+    const bool keep = (j < u.n && (j < u.lo || j >= u.hi)) || (cand && r[e] > t) ||
+                      (tie && seen + __builtin_popcountll(mt & ((1ull << lane) - 1)) < ties);
+    seen += __builtin_popcountll(mt);
+    return __builtin_amdgcn_ballot_w64(keep);
+  };
+  int mine = 0, seen = before;
+#pragma unroll
+  for (int e = 0; e < NE; ++e) {
+    mine += __builtin_popcountll(keeps(e, seen));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+  (void)block_sum(mine, counts[0]);
+  int at = 0;
+#pragma unroll
+  for (int w = 0; w < kSelThreads / 64; ++w) at += w < wave ? counts[0][w] : 0;
+  seen = before;
+#pragma unroll
+  for (int e = 0; e < NE; ++e) {
+    const uint64_t on = keeps(e, seen);
+    const int i = at + __builtin_popcountll(on & ((1ull << lane) - 1));
+    if (((on >> lane) & 1) && i < a.keep) u.out[i] = j0 + 64 * e;
+    at += __builtin_popcountll(on);
+    __builtin_amdgcn_sched_barrier(0);  // (one mask at a time)
+  }
+}
+
+// The same for sequences that registers do not hold: the weights are read
+// again for every bit.
+__global__ __launch_bounds__(kSelThreads) void select_long_kernel(const SelectArgs a) {
+  __shared__ int counts[2][kSelThreads / 64];
+  __shared__ int above[kSelThreads / 64], equal[kSelThreads / 64];
+  const SelectUnit u = select_unit(a);
+  if (u.n <= a.keep) {
+    select_all(a, u);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t t = 0xffffffffu;
+  if (u.want > 0) {
+    t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = t | (1u << bit);
+      int c = 0;
+      for (int j = u.lo + tid; j - tid < u.hi; j += kSelThreads)
+        c += wave_count(j < u.hi && rank_of(u.w[(int64_t)j * a.ws_k]) >= cand);
+      if (block_sum(c, counts[bit & 1]) >= u.want) t = cand;
+    }
+  }
+  int c = 0;
+  for (int j = u.lo + tid; j - tid < u.hi; j += kSelThreads)
+    c += wave_count(j < u.hi && u.want > 0 && rank_of(u.w[(int64_t)j * a.ws_k]) > t);
+  __syncthreads();
+  const int ties = u.want - block_sum(c, counts[0]);
+  // rows in order, 1024 at a time
   int done = 0, taken = 0;  // rows written, ties taken, before this chunk
-  for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-    const int j = j0 + tid;
-    const bool cand = want > 0 && j >= lo && j < hi;
-    const uint32_t r = cand ? rank_of(w[(int64_t)j * a.ws_k]) : 0u;
-    const bool sure = j < n && (j < lo || j >= hi || (cand && r > t)), tie = cand && r == t;
+  for (int r0 = 0; r0 < u.n; r0 += kSelThreads) {
+    const int j = r0 + tid;
+    const bool cand = u.want > 0 && j >= u.lo && j < u.hi;
+    const uint32_t r = cand ? rank_of(u.w[(int64_t)j * a.ws_k]) : 0u;
+    const bool sure = j < u.n && (j < u.lo || j >= u.hi || (cand && r > t)), tie = cand && r == t;
     const uint64_t mt = __builtin_amdgcn_ballot_w64(tie);
     if (lane == 0) equal[wave] = __builtin_popcountll(mt);
     __syncthreads();
@@ -115,11 +220,16 @@ __global__ __launch_bounds__(kSelThreads) void select_keys_kernel(const SelectAr
       sum += above[x];
     }
     at += __builtin_popcountll(mo & ((1ull << lane) - 1));
-    if (on && at < a.keep) out[at] = j;
+    if (on && at < a.keep) u.out[at] = j;
     done = sum;
     taken = all;
     __syncthreads();
   }
+}
+
+template <int NE>
+void launch_select(const SelectArgs& a, unsigned units, hipStream_t st) {
+  hipLaunchKernelGGL((select_keys_kernel<NE>), dim3(units), dim3(kSelThreads), 0, st, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -134,6 +244,7 @@ struct MoveTensor {
   int width;                                   // bytes of a row
   int unit;                                    // bytes moved at a time (16, 8, 4, 2 or 1)
   int lpr;                                     // units of a row
+  FastDiv div;                                 // by lpr
 };
 
 struct MoveArgs {
@@ -145,6 +256,7 @@ struct MoveArgs {
   int64_t S, dst_rows;
   PageMap pm;  // paged: source and destination rows go through the table
   int H, n;
+  uint32_t wg0[kMoveMax];  // first workgroup of each tensor (none: past the last)
 };
 
 __device__ __forceinline__ int64_t move_first(const MoveArgs& a, int b) { return a.first ? a.first[b] : a.first0; }
@@ -185,21 +297,37 @@ __device__ __forceinline__ void move_store(uint8_t* p, int unit, uint4 v) {
 }
 
 constexpr int kMoveThreads = 256;
+constexpr int kMovePer = 4;  // pieces a thread moves, all loads before the stores
 
-// Into other buffers: a thread moves one piece of one row; blockIdx.y is the
-// tensor, blockIdx.z the (sequence, head).
+// Into other buffers: a thread moves pieces of rows; a workgroup's tensor is
+// found from the workgroups of those before it, blockIdx.y is the (sequence,
+// head). Memory-bound, in pieces of up to 16 bytes of rows that lie apart.
 __global__ __launch_bounds__(kMoveThreads) void move_rows_kernel(const MoveArgs a) {
-  const MoveTensor t = a.t[blockIdx.y];
-  const int h = blockIdx.z % a.H, b = blockIdx.z / a.H;
-  const int64_t x = (int64_t)blockIdx.x * kMoveThreads + threadIdx.x;
-  const int64_t i = x / t.lpr;
-  if (i >= a.n) return;
-  const int at = (int)(x % t.lpr) * t.unit;
-  int64_t s, d;
-  move_rows_of(a, b, h, (int)i, &s, &d);
-  if (s < 0) return;
-  move_store(t.dst + b * t.ds_b + h * t.ds_h + d * t.ds_s + at, t.unit,
-             move_load(t.src + b * t.ss_b + h * t.ss_h + s * t.ss_s + at, t.unit));
+  int k = 0;
+#pragma unroll
+  for (int x = 1; x < kMoveMax; ++x) k = blockIdx.x >= a.wg0[x] ? x : k;
+  const MoveTensor& t = a.t[k];
+  const int h = blockIdx.y % a.H, b = blockIdx.y / a.H;
+  const uint32_t x0 = (blockIdx.x - a.wg0[k]) * (kMoveThreads * kMovePer) + threadIdx.x;
+  const uint32_t pieces = (uint32_t)a.n * (uint32_t)t.lpr;
+  int64_t s[kMovePer], d[kMovePer];
+  int at[kMovePer];
+#pragma unroll
+  for (int y = 0; y < kMovePer; ++y) {
+    const uint32_t x = x0 + y * kMoveThreads, i = fdiv(x, t.div);
+    at[y] = (int)(x - i * (uint32_t)t.lpr) * t.unit;
+    s[y] = -1;
+    if (x < pieces) move_rows_of(a, b, h, (int)i, &s[y], &d[y]);
+  }
+  const uint8_t* src = t.src + b * t.ss_b + h * t.ss_h;
+  uint8_t* dst = t.dst + b * t.ds_b + h * t.ds_h;
+  uint4 v[kMovePer];
+#pragma unroll
+  for (int y = 0; y < kMovePer; ++y)
+    if (s[y] >= 0) v[y] = move_load(src + s[y] * t.ss_s + at[y], t.unit);
+#pragma unroll
+  for (int y = 0; y < kMovePer; ++y)
+    if (s[y] >= 0) move_store(dst + d[y] * t.ds_s + at[y], t.unit, v[y]);
 }
 
 // In place: one workgroup per tensor, sequence and head reads every row that
@@ -241,7 +369,8 @@ int move_impl(const char* what, int64_t n_tensors, const void* const* src, const
                 "%s: bad shape (B=%lld H=%lld S=%lld n=%lld)", what, (long long)B, (long long)H, (long long)S,
                 (long long)n);
   MoveArgs a = {};
-  int64_t most = 0;
+  int64_t wgs = 0;
+  for (int k = 0; k < kMoveMax; ++k) a.wg0[k] = 0xffffffffu;
   for (int k = 0; k < n_tensors; ++k) {
     const int64_t* ss = src_strides + 3 * k;
     const int64_t* ds = dst_strides + 3 * k;
@@ -261,9 +390,12 @@ int move_impl(const char* what, int64_t n_tensors, const void* const* src, const
     };
     while (t.unit > 1 && !fits(t.unit)) t.unit >>= 1;
     t.lpr = t.width / t.unit;
+    t.div = make_fastdiv((uint32_t)t.lpr);
     if (in_place) KVQ_CHECK_ARG(n * widths[k] <= kMoveLds, "%s: in place, at most %d bytes of rows a head move (got %lld)",
                                 what, kMoveLds, (long long)(n * widths[k]));
-    most = n * t.lpr > most ? n * t.lpr : most;
+    KVQ_CHECK_ARG(n * t.lpr < (int64_t(1) << 31), "%s: too large", what);
+    a.wg0[k] = (uint32_t)wgs;
+    wgs += (n * t.lpr + kMoveThreads * kMovePer - 1) / (kMoveThreads * kMovePer);
   }
   if (B == 0 || n == 0) return KVQ_OK;
   KVQ_CHECK_ARG(index, "%s: null index", what);
@@ -281,10 +413,8 @@ int move_impl(const char* what, int64_t n_tensors, const void* const* src, const
     hipLaunchKernelGGL(move_rows_in_place_kernel, dim3(1, (unsigned)n_tensors, (unsigned)(B * H)), dim3(kMoveThreads), 0,
                        st, a);
   } else {
-    const int64_t wgs = (most + kMoveThreads - 1) / kMoveThreads;
     KVQ_CHECK_ARG(wgs < (int64_t(1) << 31), "%s: too large", what);
-    hipLaunchKernelGGL(move_rows_kernel, dim3((unsigned)wgs, (unsigned)n_tensors, (unsigned)(B * H)), dim3(kMoveThreads),
-                       0, st, a);
+    hipLaunchKernelGGL(move_rows_kernel, dim3((unsigned)wgs, (unsigned)(B * H)), dim3(kMoveThreads), 0, st, a);
   }
   KVQ_CHECK_LAUNCH(what);
   return KVQ_OK;
@@ -310,7 +440,14 @@ extern "C" int kvq_select_keys(const float* weights, const int64_t* weight_strid
   KVQ_CHECK_ARG(index && (weights || S == 0), "kvq_select_keys: null data pointer");
   const SelectArgs a = {weights, weight_strides[0], weight_strides[1], weight_strides[2], index, seq_lens, S, (int)H,
                         (int)n_keep, (int)sink, (int)recent};
-  hipLaunchKernelGGL(select_keys_kernel, dim3((unsigned)(B * H)), dim3(kSelThreads), 0, (hipStream_t)stream, a);
+  const unsigned units = (unsigned)(B * H);
+  hipStream_t st = (hipStream_t)stream;
+  if (S <= 2 * kSelThreads) launch_select<2>(a, units, st);
+  else if (S <= 8 * kSelThreads) launch_select<8>(a, units, st);
+  else if (S <= 16 * kSelThreads) launch_select<16>(a, units, st);
+  else if (S <= 32 * kSelThreads) launch_select<32>(a, units, st);
+  else if (S <= 64 * kSelThreads) launch_select<64>(a, units, st);
+  else hipLaunchKernelGGL(select_long_kernel, dim3(units), dim3(kSelThreads), 0, st, a);
   KVQ_CHECK_LAUNCH("kvq_select_keys");
   return KVQ_OK;
 }
