@@ -27,17 +27,14 @@ struct SelectArgs {
   int keep, sink, recent;
 };
 
-constexpr int kSelThreads = 1024;
-
-// Weights in the order of their floats: NaN above everything, -0 as +0.
+// Weights in the order of their floats: NaN above every number, -0 as +0. No
+// weight has rank 0 (no row) or 0xffffffff (a row that is always kept).
 __device__ __forceinline__ uint32_t rank_of(float x) {
   uint32_t u = __builtin_bit_cast(uint32_t, x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xfffffffeu;
   if (u == 0x80000000u) u = 0u;
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-
-__device__ __forceinline__ int wave_count(bool x) { return __builtin_popcountll(__builtin_amdgcn_ballot_w64(x)); }
 
 struct SelectUnit {
   const float* w;
@@ -63,173 +60,153 @@ __device__ __forceinline__ SelectUnit select_unit(const SelectArgs& a) {
 }
 
 // A sequence that keeps everything.
+template <int NT>
 __device__ __forceinline__ void select_all(const SelectArgs& a, const SelectUnit& u) {
-  for (int i = threadIdx.x; i < a.keep; i += kSelThreads) u.out[i] = i < u.n ? i : -1;
+  for (int i = threadIdx.x; i < a.keep; i += NT) u.out[i] = i < u.n ? i : -1;
 }
 
-// Sum over the workgroup's waves of a value uniform in each wave; `slot`
-// alternates between two calls' buffers, so that one barrier is enough.
-__device__ __forceinline__ int block_sum(int x, int* slot) {
-  if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < kSelThreads / 64; ++w) total += slot[w];
-  return total;
+// x + the value `lanes` lanes below, by DPP (0 where there is none): control
+// words row_shr 1, 2, 4, 8 (within 16 lanes), then row 15's and row 31's last
+// lane to the rows above.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int row_prefix(int x) {  // inclusive sum over each 16 lanes
+  x = dpp_add<0x111, 0xf>(x);
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  return dpp_add<0x118, 0xf>(x);
+}
+__device__ __forceinline__ int wave_prefix(int x) {  // over the wave
+  x = dpp_add<0x142, 0xa>(row_prefix(x));
+  return dpp_add<0x143, 0xc>(x);
 }
 
-// One workgroup per (sequence, KV head), its ranks in registers (NE a thread;
-// each wave holds 64 NE consecutive rows, so that its kept rows are counted
-// and written in order). The rank of the want-th largest is built bit by bit
-// from the top: a bit is set if that many candidates are at least the rank so
-// formed, counted with one compare a register and ballots (a histogram in LDS
-// would put most of a wave's lanes on the same few exponents). It stops as soon
-// as exactly `want` candidates are at or above it. Bound by those compares and a
-// barrier a bit, about 0.2 us a bit at 16K keys.
-template <int NE>
-__global__ __launch_bounds__(kSelThreads) void select_keys_kernel(const SelectArgs a) {
-  __shared__ int counts[2][kSelThreads / 64];
+// One workgroup of NT threads per (sequence, KV head). The rank of the last row
+// kept is found six bits a round from the top: the rows that share its bits so
+// far are counted by their next six, in LDS, in 16 columns (a wave's lanes mostly
+// have the same few exponents; in one counter they would wait for each other),
+// and the columns added up. It stops as soon as a count
+// is exactly what is wanted: after four rounds for weights that spread over the
+// floats. Then the kept rows are counted and written in order, each wave a run
+// of consecutive rows. Ranks are kept in LDS between the passes (up to CAP
+// rows; CAP 0: formed again from the weights each time). Loops stay rolled: a
+// few workgroups run this code once, and unrolled over ranks in registers most
+// of the time went by until the instructions arrived (16K rows: 31 us so, of
+// which the last pass alone took 20).
+constexpr int kBits = 6, kBins = 1 << kBits;
+
+template <int NT, int CAP>
+__global__ __launch_bounds__(NT) void select_keys_kernel(const SelectArgs a) {
+  constexpr int NW = NT / 64;
+  __shared__ uint32_t ranks[CAP > 0 ? CAP : 1];
+  __shared__ int hist[kBins * 16];
+  __shared__ int totals[kBins];
+  __shared__ int counts[2][NW];
   const SelectUnit u = select_unit(a);
   if (u.n <= a.keep) {
-    select_all(a, u);
+    select_all<NT>(a, u);
     return;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int j0 = wave * (64 * NE) + lane;
-  uint32_t r[NE];  // ranks of rows j0 + 64 e; 0 (below every rank) outside the candidates
-#pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    const int j = j0 + 64 * e;
-    r[e] = j >= u.lo && j < u.hi ? rank_of(u.w[(int64_t)j * a.ws_k]) : 0u;
-  }
-  uint32_t t = 0;
-  bool exact = u.want == 0;  // whether the candidates at or above t are just those kept
-  if (!exact) {
-#pragma unroll 1
-    for (int bit = 31; bit >= 0 && !exact; --bit) {
-      const uint32_t cand = t | (1u << bit);
-      int c = 0;
-#pragma unroll
-      for (int e = 0; e < NE; ++e) c += wave_count(r[e] >= cand);
-      const int total = block_sum(c, counts[bit & 1]);
-      if (total >= u.want) {
-        t = cand;
-        exact = total == u.want;
-      }
-    }
-  } else {
-    t = 0xffffffffu;
-  }
-  // of the candidates that equal t, the first `ties` (exact: all of them)
-  int above = 0, equal = 0;
-#pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    above += wave_count(r[e] > t);
-    equal += wave_count(r[e] == t && t != 0u);
-  }
-  if (u.want == 0) above = equal = 0;
-  __syncthreads();
-  const int all_above = block_sum(above, counts[0]);
-  int ties = u.want - all_above, before = 0;
-  (void)block_sum(equal, counts[1]);
-#pragma unroll
-  for (int w = 0; w < kSelThreads / 64; ++w) before += w < wave ? counts[1][w] : 0;
-  // rows kept in this wave, its place among the waves', then the rows again
-  auto keeps = [&](int e, int& seen) {  // the wave's kept rows among its e-th 64; seen: ties so far
-    const int j = j0 + 64 * e;
-    const bool cand = u.want > 0 && j >= u.lo && j < u.hi;
-    const bool tie = cand && r[e] == t;
-    const uint64_t mt = __builtin_amdgcn_ballot_w64(tie);
-    const bool keep = (j < u.n && (j < u.lo || j >= u.hi)) || (cand && r[e] > t) ||
-                      (tie && seen + __builtin_popcountll(mt & ((1ull << lane) - 1)) < ties);
-    seen += __builtin_popcountll(mt);
-    return __builtin_amdgcn_ballot_w64(keep);
+  // the rank of row j; always kept: the largest, past the sequence: 0
+  auto rank_from = [&](int j, float w) {
+    const uint32_t x = j < u.lo || j >= u.hi ? 0xffffffffu : rank_of(w);
+    return j < u.n ? x : 0u;
   };
-  int mine = 0, seen = before;
+  auto load = [&](int j) { return u.w[(int64_t)min(j, u.n - 1) * a.ws_k]; };
+  const int per = (u.n + NT - 1) / NT;  // 64-row pieces of a wave
+  const int j0 = wave * (64 * per) + lane;
+  for (int x = threadIdx.x; x < kBins * 16; x += NT) hist[x] = 0;
+  if constexpr (CAP > 0) {
+    int e = 0;
+    for (; e + 8 <= per; e += 8) {  // (eight loads in flight)
+      float w[8];
 #pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    mine += __builtin_popcountll(keeps(e, seen));
-    __builtin_amdgcn_sched_barrier(0);
+      for (int k = 0; k < 8; ++k) w[k] = load(j0 + 64 * (e + k));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ranks[j0 + 64 * (e + k)] = rank_from(j0 + 64 * (e + k), w[k]);
+    }
+    for (; e < per; ++e) ranks[j0 + 64 * e] = rank_from(j0 + 64 * e, load(j0 + 64 * e));
+  }
+  auto rank_at = [&](int e) {
+    const int j = j0 + 64 * e;
+    if constexpr (CAP > 0) return ranks[j];
+    else return rank_from(j, load(j));
+  };
+  __syncthreads();
+  uint32_t t = 0;       // the rank's bits so far
+  int need = a.keep;    // rows to keep among those that share them
+  bool exact = false;   // whether all of those are kept
+#pragma unroll 1
+  for (int shift = 32 - kBits; !exact; shift -= kBits) {
+    const int sh = shift > 0 ? shift : 0;
+    const uint32_t low = shift > 0 ? kBins - 1 : (1u << (kBits + shift)) - 1;  // (fewer bits in the last round)
+#pragma unroll 4
+    for (int e = 0; e < per; ++e) {
+      const uint32_t x = rank_at(e) >> sh;
+      if (((x ^ (t >> sh)) & ~low) == 0) atomicAdd(&hist[(x & low) * 16 + (lane & 15)], 1);
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < kBins * 16; x += NT) {
+      const int v = row_prefix(hist[x]);
+      hist[x] = 0;
+      if ((x & 15) == 15) totals[x >> 4] = v;
+    }
+    __syncthreads();
+    const int mine = totals[kBins - 1 - lane];  // bins from the top
+    const int sum = wave_prefix(mine);
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum >= need));
+    const int bin = __builtin_amdgcn_readlane(mine, at);
+    need -= __builtin_amdgcn_readlane(sum, at) - bin;
+    t |= (uint32_t)(kBins - 1 - at) << sh;
+    exact = need == bin;
+    if (shift <= 0) break;
+  }
+  // kept: ranks over t, and `need` of those equal to it (exact: t is lowered so
+  // that all its rows are over it; no rank of a row is 0)
+  if (exact) t -= 1;
+  int above = 0, equal = 0;
+#pragma unroll 4
+  for (int e = 0; e < per; ++e) {
+    const uint32_t r = rank_at(e);
+    above += r > t ? 1 : 0;
+    equal += r == t ? 1 : 0;
+  }
+  above = __builtin_amdgcn_readlane(wave_prefix(above), 63);
+  equal = exact ? 0 : __builtin_amdgcn_readlane(wave_prefix(equal), 63);
+  if (lane == 0) {
+    counts[0][wave] = above;
+    counts[1][wave] = equal;
   }
   __syncthreads();
-  (void)block_sum(mine, counts[0]);
-  int at = 0;
-#pragma unroll
-  for (int w = 0; w < kSelThreads / 64; ++w) at += w < wave ? counts[0][w] : 0;
-  seen = before;
-#pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    const uint64_t on = keeps(e, seen);
-    const int i = at + __builtin_popcountll(on & ((1ull << lane) - 1));
-    if (((on >> lane) & 1) && i < a.keep) u.out[i] = j0 + 64 * e;
-    at += __builtin_popcountll(on);
-    __builtin_amdgcn_sched_barrier(0);  // (one mask at a time)
+  int at = 0, seen = 0;  // rows kept, and rows equal to t, before this wave's
+  for (int x = 0; x < wave; ++x) {
+    at += counts[0][x];
+    seen += counts[1][x];
+  }
+  at = __builtin_amdgcn_readfirstlane(at + min(seen, need));
+  seen = __builtin_amdgcn_readfirstlane(seen);
+#pragma unroll 2
+  for (int e = 0; e < per; ++e) {
+    const uint32_t r = rank_at(e);
+    bool on = r > t;
+    if (!exact) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64(r == t);
+      on = on || (r == t && seen + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)) < need);
+      seen += __builtin_popcountll(m);
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(on);
+    const int i = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    if (on && i < a.keep) u.out[i] = j0 + 64 * e;
+    at += __builtin_popcountll(m);
   }
 }
 
-// The same for sequences that registers do not hold: the weights are read
-// again for every bit.
-__global__ __launch_bounds__(kSelThreads) void select_long_kernel(const SelectArgs a) {
-  __shared__ int counts[2][kSelThreads / 64];
-  __shared__ int above[kSelThreads / 64], equal[kSelThreads / 64];
-  const SelectUnit u = select_unit(a);
-  if (u.n <= a.keep) {
-    select_all(a, u);
-    return;
-  }
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint32_t t = 0xffffffffu;
-  if (u.want > 0) {
-    t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t cand = t | (1u << bit);
-      int c = 0;
-      for (int j = u.lo + tid; j - tid < u.hi; j += kSelThreads)
-        c += wave_count(j < u.hi && rank_of(u.w[(int64_t)j * a.ws_k]) >= cand);
-      if (block_sum(c, counts[bit & 1]) >= u.want) t = cand;
-    }
-  }
-  int c = 0;
-  for (int j = u.lo + tid; j - tid < u.hi; j += kSelThreads)
-    c += wave_count(j < u.hi && u.want > 0 && rank_of(u.w[(int64_t)j * a.ws_k]) > t);
-  __syncthreads();
-  const int ties = u.want - block_sum(c, counts[0]);
-  // rows in order, 1024 at a time
-  int done = 0, taken = 0;  // rows written, ties taken, before this chunk
-  for (int r0 = 0; r0 < u.n; r0 += kSelThreads) {
-    const int j = r0 + tid;
-    const bool cand = u.want > 0 && j >= u.lo && j < u.hi;
-    const uint32_t r = cand ? rank_of(u.w[(int64_t)j * a.ws_k]) : 0u;
-    const bool sure = j < u.n && (j < u.lo || j >= u.hi || (cand && r > t)), tie = cand && r == t;
-    const uint64_t mt = __builtin_amdgcn_ballot_w64(tie);
-    if (lane == 0) equal[wave] = __builtin_popcountll(mt);
-    __syncthreads();
-    int before = taken, all = taken;
-    for (int x = 0; x < kSelThreads / 64; ++x) {
-      if (x < wave) before += equal[x];
-      all += equal[x];
-    }
-    before += __builtin_popcountll(mt & ((1ull << lane) - 1));
-    const bool on = sure || (tie && before < ties);
-    const uint64_t mo = __builtin_amdgcn_ballot_w64(on);
-    if (lane == 0) above[wave] = __builtin_popcountll(mo);
-    __syncthreads();
-    int at = done, sum = done;
-    for (int x = 0; x < kSelThreads / 64; ++x) {
-      if (x < wave) at += above[x];
-      sum += above[x];
-    }
-    at += __builtin_popcountll(mo & ((1ull << lane) - 1));
-    if (on && at < a.keep) u.out[at] = j;
-    done = sum;
-    taken = all;
-    __syncthreads();
-  }
-}
-
-template <int NE>
+template <int NT, int CAP>
 void launch_select(const SelectArgs& a, unsigned units, hipStream_t st) {
-  hipLaunchKernelGGL((select_keys_kernel<NE>), dim3(units), dim3(kSelThreads), 0, st, a);
+  hipLaunchKernelGGL((select_keys_kernel<NT, CAP>), dim3(units), dim3(NT), 0, st, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -442,12 +419,12 @@ extern "C" int kvq_select_keys(const float* weights, const int64_t* weight_strid
                         (int)n_keep, (int)sink, (int)recent};
   const unsigned units = (unsigned)(B * H);
   hipStream_t st = (hipStream_t)stream;
-  if (S <= 2 * kSelThreads) launch_select<2>(a, units, st);
-  else if (S <= 8 * kSelThreads) launch_select<8>(a, units, st);
-  else if (S <= 16 * kSelThreads) launch_select<16>(a, units, st);
-  else if (S <= 32 * kSelThreads) launch_select<32>(a, units, st);
-  else if (S <= 64 * kSelThreads) launch_select<64>(a, units, st);
-  else hipLaunchKernelGGL(select_long_kernel, dim3(units), dim3(kSelThreads), 0, st, a);
+  // as few waves as keep a few rows each busy (every wave repeats the rounds'
+  // bookkeeping), and no more LDS than the rows need
+  if (S <= 2048) launch_select<256, 2048>(a, units, st);
+  else if (S <= 8192) launch_select<512, 8192>(a, units, st);
+  else if (S <= 32768) launch_select<1024, 32768>(a, units, st);
+  else launch_select<1024, 0>(a, units, st);
   KVQ_CHECK_LAUNCH("kvq_select_keys");
   return KVQ_OK;
 }
