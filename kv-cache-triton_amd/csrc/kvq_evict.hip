@@ -368,6 +368,18 @@ int move_impl(const char* what, int64_t n_tensors, const void* const* src, const
     while (t.unit > 1 && !fits(t.unit)) t.unit >>= 1;
     t.lpr = t.width / t.unit;
     t.div = make_fastdiv((uint32_t)t.lpr);
+    if (!in_place) {  // no destination may overlap a source
+      auto last = [](const int64_t* st, int64_t B, int64_t H, int64_t rows, int64_t width) {
+        return (B - 1) * st[0] + (H - 1) * st[1] + (rows - 1) * st[2] + width;
+      };
+      for (int x = 0; x < n_tensors && B > 0 && S > 0 && dst_rows > 0; ++x) {
+        const uint8_t* s0 = (const uint8_t*)src[x];
+        const uint8_t* d0 = (const uint8_t*)dst[k];
+        KVQ_CHECK_ARG(d0 + last(ds, B, H, dst_rows, widths[k]) <= s0 ||
+                          s0 + last(src_strides + 3 * x, B, H, S, widths[x]) <= d0,
+                      "%s: a destination overlaps a tensor that is read (in_place moves within one)", what);
+      }
+    }
     if (in_place) KVQ_CHECK_ARG(n * widths[k] <= kMoveLds, "%s: in place, at most %d bytes of rows a head move (got %lld)",
                                 what, kMoveLds, (long long)(n * widths[k]));
     KVQ_CHECK_ARG(n * t.lpr < (int64_t(1) << 31), "%s: too large", what);

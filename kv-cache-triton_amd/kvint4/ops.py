@@ -1030,17 +1030,30 @@ def _check_cache(what: str, q: torch.Tensor, caches: tuple, B: int, Hkv: int, D:
         raise ValueError("group_size must be > 0")
     if Hkv < 1 or q.shape[1] % Hkv:
         raise ValueError(f"the query heads ({q.shape[1]}) must be a multiple of n_kv_heads ({Hkv})")
-    S = caches[0].shape[2] if caches[0].dim() == 4 else -1
-    for codes, scales in zip(caches[0::2], caches[1::2]):
-        if codes.dim() != 4 or scales.dim() != 4 or codes.shape[:3] != (B, Hkv, S) or scales.shape[:3] != (B, Hkv, S):
+    lead = (B, Hkv, caches[0].shape[2] if caches[0].dim() == 4 else -1)
+    sdt, w, ng = caches[1].dtype, packed_width(D, group_size), num_groups(D, group_size)
+    if sdt not in SUPPORTED_FLOATS:
+        raise ValueError(f"{what}: scales must be bf16/fp16/fp32")
+    for t, dt, width in zip(caches, (torch.uint8, sdt) * 2, (w, ng) * 2):
+        shape = t.shape
+        if len(shape) != 4 or shape[:3] != lead:
             raise ValueError(f"{what}: codes and scales must be [B={B}, n_kv_heads={Hkv}, Sk, .] of one Sk "
-                             f"(got {tuple(codes.shape)}, {tuple(scales.shape)})")
-        if codes.dtype != torch.uint8 or scales.dtype not in SUPPORTED_FLOATS or scales.dtype != caches[1].dtype:
-            raise ValueError(f"{what}: codes must be uint8, scales bf16/fp16/fp32 of one dtype")
-        if codes.shape[-1] < packed_width(D, group_size) or scales.shape[-1] < num_groups(D, group_size):
+                             f"(got {tuple(shape)})")
+        if t.dtype != dt:
+            raise ValueError(f"{what}: codes must be uint8, scales of one dtype (got {t.dtype})")
+        if shape[3] < width:
             raise ValueError(f"{what}: cache last dims are too small for this head dim / group size")
-        if codes.stride(-1) != 1 or scales.stride(-1) != 1:
+        if t.stride(3) != 1:
             raise ValueError(f"{what}: cache last dims must be contiguous")
+
+
+def _one_device(what: str, dev: int, ts) -> None:
+    """Every tensor of `ts` on GPU `dev` (a device index)."""
+    for t in ts:
+        if t.get_device() != dev or dev < 0:
+            if dev < 0 or t.get_device() < 0:
+                raise ValueError(f"{what} expects GPU tensors (got a tensor on {t.device if dev >= 0 else 'cpu'})")
+            raise ValueError(f"{what}: every tensor must be on one device (GPU {dev}; got one on {t.device})")
 
 
 def _check_block(what: str, q: torch.Tensor, out: torch.Tensor | None, *others: torch.Tensor) -> torch.Tensor:
@@ -1048,14 +1061,13 @@ def _check_block(what: str, q: torch.Tensor, out: torch.Tensor | None, *others: 
     holds every operand: `out`, or a new tensor."""
     if q.dim() != 4 or q.dtype not in SUPPORTED_FLOATS:
         raise ValueError(f"{what}: q must be [B, Hq, Sq, D] in bf16/fp16/fp32")
+    _one_device(what, q.get_device(), others)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError(f"{what}: out must have q's shape and dtype")
-    _check_cuda(q, out, *others, what=what)
-    for t in (out, *others):
-        if t.get_device() != q.get_device():
-            raise ValueError(f"{what}: every tensor must be on q's device ({q.device}; got one on {t.device})")
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out is not q:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"{what}: out must have q's shape and dtype")
+        _one_device(what, q.get_device(), (out,))
     return out
 
 
@@ -1297,7 +1309,7 @@ def select_keys(
     B, H, S = key_weights.shape
     if key_weights.dtype != torch.float32:
         raise ValueError(f"{what}: key_weights must be fp32 (got {key_weights.dtype})")
-    _check_cuda(key_weights, what=what)
+    _one_device(what, key_weights.get_device(), (key_weights,))
     if seq_len is not None:
         if not 0 <= int(seq_len) <= S:
             raise ValueError(f"{what}: seq_len {seq_len} outside [0, {S}]")
@@ -1315,38 +1327,24 @@ def select_keys(
     return index
 
 
-def _check_index(what: str, index: torch.Tensor, B: int, H: int, device: torch.device) -> torch.Tensor:
+def _check_index(what: str, index: torch.Tensor, B: int, H: int) -> torch.Tensor:
     """index [B or 1, H or 1, n] as [B, H, n] (stride 0 where shared)."""
     if index.dtype != torch.int32 or index.dim() != 3 or index.shape[0] not in (1, B) or index.shape[1] not in (1, H):
         raise ValueError(f"{what}: index must be int32 [B={B} or 1, H={H} or 1, n] (got {index.dtype} "
                          f"{tuple(index.shape)})")
-    if index.device != device:
-        raise ValueError(f"{what}: index must be on the tensors' device ({device}; got {index.device})")
-    return index.expand(B, H, index.shape[2])
+    return index if index.shape[:2] == (B, H) else index.expand(B, H, index.shape[2])
 
 
-def _first(what: str, first, B: int, device: torch.device) -> tuple:
+def _first(what: str, first, B: int, dev: int) -> tuple:
     """(pointer or None, scalar, the tensor behind the pointer) of the first destination row."""
     if not isinstance(first, torch.Tensor):
         if int(first) < 0:
             raise ValueError(f"{what}: first must be >= 0")
         return None, int(first), None
-    if first.dtype != torch.int32 or first.numel() != B or first.device != device:
+    if first.dtype != torch.int32 or first.numel() != B or first.get_device() != dev:
         raise ValueError(f"{what}: first must be an int or an int32 tensor [B] on the tensors' device")
     first = first.contiguous()
     return first.data_ptr(), 0, first
-
-
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """[first, last) byte addresses that a tensor's elements lie in."""
-    if t.numel() == 0:
-        return t.data_ptr(), t.data_ptr()
-    n = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (n + 1) * t.element_size()
-
-
-def _row_bytes(t: torch.Tensor) -> int:
-    return t.element_size() * (t.shape[3] if t.dim() == 4 else 1)
 
 
 # Bytes of rows per tensor and head that move in place (the workgroup holds
@@ -1365,39 +1363,37 @@ def move_rows(tensors, index: torch.Tensor, *, out=None, first=0) -> None:
     rows that nothing moves to are left as they are."""
     what = "move_rows"
     tensors = tuple(tensors)
+    dst = tensors if out is None else tuple(out)
     if not 1 <= len(tensors) <= 5 or any(t.dim() not in (3, 4) for t in tensors):
         raise ValueError(f"{what}: 1 to 5 tensors [B, H, S, w] or [B, H, S]")
-    dst = tensors if out is None else tuple(out)
     if len(dst) != len(tensors):
         raise ValueError(f"{what}: out must hold a destination for every tensor")
-    _check_cuda(*tensors, *dst, index, what=what)
-    B, H, S = tensors[0].shape[:3]
-    dev, rows = tensors[0].device, dst[0].shape[2] if dst[0].dim() in (3, 4) else -1
-    for t, d in zip(tensors, dst):
-        if t.shape[:3] != (B, H, S) or d.dim() != t.dim() or d.shape[:3] != (B, H, rows) or d.shape[3:] != t.shape[3:] \
-                or d.dtype != t.dtype:
-            raise ValueError(f"{what}: tensors must share [B, H, S], and out's match them but for the rows "
-                             f"(got {tuple(t.shape)} {t.dtype} -> {tuple(d.shape)} {d.dtype})")
-        if t.device != dev or d.device != dev:
-            raise ValueError(f"{what}: every tensor must be on one device")
-        if t.dim() == 4 and (t.stride(3) != 1 or d.stride(3) != 1):
-            raise ValueError(f"{what}: rows must be contiguous")
+    lead = B, H, S = tuple(tensors[0].shape[:3])
+    dev, rows = index.get_device(), dst[0].shape[2] if dst[0].dim() in (3, 4) else -1
+    _one_device(what, dev, tensors)
     if out is not None:
-        spans = [_span(t) for t in tensors]
-        for d in dst:
-            lo, hi = _span(d)
-            if any(lo < h and l < hi for l, h in spans):
-                raise ValueError(f"{what}: out overlaps the tensors that it is read from")
-    index = _check_index(what, index, B, H, dev)
+        _one_device(what, dev, dst)
+    sizes, widths = [], []
+    for t, d in zip(tensors, dst):
+        shape = t.shape
+        if shape[:3] != lead or (d is not t and (d.shape != (B, H, rows, *shape[3:]) or d.dtype != t.dtype)):
+            raise ValueError(f"{what}: tensors must share [B, H, S], and out's match them but for the rows "
+                             f"(got {tuple(shape)} {t.dtype} -> {tuple(d.shape)} {d.dtype})")
+        size, width = t.element_size(), 1
+        if len(shape) == 4:
+            width = shape[3]
+            if t.stride(3) != 1 or d.stride(3) != 1:
+                raise ValueError(f"{what}: rows must be contiguous")
+        sizes.append(size)
+        widths.append(size * width)
+    index = _check_index(what, index, B, H)
     first_ptr, first0, first = _first(what, first, B, dev)
     n = index.shape[2]
-    if B == 0 or H == 0 or n == 0 or any(_row_bytes(t) == 0 for t in tensors):
+    if B == 0 or H == 0 or n == 0 or 0 in widths:
         return
     with nat.device_of(index) as stream:
-        rc = nat.host().move_rows(
-            tensors, dst, tuple(t.element_size() for t in tensors), tuple(_row_bytes(t) for t in tensors), index,
-            B, H, S, n, rows, first_ptr, first0, 1 if out is None else 0, stream,
-        )
+        rc = nat.host().move_rows(tensors, dst, tuple(sizes), tuple(widths), index, B, H, S, n, rows, first_ptr, first0,
+                                  1 if out is None else 0, stream)
     nat.check(rc, "kvq_move_rows")
 
 
@@ -1410,21 +1406,20 @@ def move_rows_paged(pools, pt: PageTable, index: torch.Tensor, *, first=0) -> No
     pools = tuple(pools)
     if not 1 <= len(pools) <= 5:
         raise ValueError(f"{what}: 1 to 5 pools")
-    _check_cuda(*pools, index, pt.table, what=what)
+    dev = index.get_device()
+    _one_device(what, dev, (*pools, pt.table))
     H, rows = pools[0].shape[0], pt.num_blocks * pt.page_size
     for p in pools:
         if p.dim() != 3 or p.shape[:2] != (H, rows) or p.stride(2) != 1:
             raise ValueError(f"{what}: pools must be [H={H}, num_blocks*page_size={rows}, w] with contiguous rows "
                              f"(got {tuple(p.shape)})")
-        if p.device != pt.table.device:
-            raise ValueError(f"{what}: every tensor must be on one device")
     if index.dim() != 3:
         raise ValueError(f"{what}: index must be int32 [B, H or 1, n]")
     B = index.shape[0]
     if pt.table.shape[0] < B:
         raise ValueError("block table has fewer rows than the batch")
-    index = _check_index(what, index, B, H, pools[0].device)
-    first_ptr, first0, first = _first(what, first, B, pools[0].device)
+    index = _check_index(what, index, B, H)
+    first_ptr, first0, first = _first(what, first, B, dev)
     n = index.shape[2]
     if B == 0 or H == 0 or n == 0 or any(p.shape[2] == 0 for p in pools):
         return
