@@ -372,7 +372,7 @@ int move_impl(const char* what, int64_t n_tensors, const void* const* src, const
       auto last = [](const int64_t* st, int64_t B, int64_t H, int64_t rows, int64_t width) {
         return (B - 1) * st[0] + (H - 1) * st[1] + (rows - 1) * st[2] + width;
       };
-      for (int x = 0; x < n_tensors && B > 0 && S > 0 && dst_rows > 0; ++x) {
+      for (int x = 0; x < n_tensors && B > 0 && S > 0 && n > 0 && dst_rows > 0; ++x) {
         const uint8_t* s0 = (const uint8_t*)src[x];
         const uint8_t* d0 = (const uint8_t*)dst[k];
         KVQ_CHECK_ARG(d0 + last(ds, B, H, dst_rows, widths[k]) <= s0 ||

@@ -26,6 +26,7 @@ from typing import Optional
 import torch
 
 from . import _native, ops
+from .tree_drafts import TreeDrafts, check_paths, path_index
 
 _ROUND = 256  # capacity granularity (tokens)
 
@@ -62,7 +63,7 @@ def _round_up(n: int, m: int) -> int:
     return (n + m - 1) // m * m
 
 
-class QuantizedKVCacheBase:
+class QuantizedKVCacheBase(TreeDrafts):
     """Family-independent part of the INT4 cache. Subclasses set
     ``_scale_dtype_for(x)`` and ``_deq_dtype_default``."""
 
@@ -267,6 +268,51 @@ class QuantizedKVCacheBase:
         layer.seq_len = start + 1
         self.fused_steps += 1
         return out
+
+    # -- trees of drafted tokens -----------------------------------------------
+    def attend_tree(self, query_states: torch.Tensor, layer_idx: int, tree_mask: torch.Tensor, *, n_kv_heads: int,
+                    scale: float) -> torch.Tensor:
+        """Attention of a tree of T drafts, query_states [B, H_q, T, d], whose
+        rows are the last T of each sequence (appended before the call)."""
+        layer = self._layers[layer_idx]
+        n = layer.seq_len
+        return ops.tree_attention(
+            query_states, layer.k_packed[:, :, :n], layer.k_scales[:, :, :n], layer.v_packed[:, :, :n],
+            layer.v_scales[:, :, :n], tree_mask, n_kv_heads=n_kv_heads, group_size=self.group_size, sm_scale=scale,
+            seq_lens=layer.seq_lens)
+
+    def accept(self, block: int, paths) -> None:
+        """Of the last `block` tokens of each sequence, in every layer, keep the
+        accepted ones: paths[b], ascending places in the block (a tree's
+        verified path; none: an empty list). Their rows move to the front of
+        the block and the others are dropped. Sequences that accept different
+        numbers of tokens become a ragged batch."""
+        if not self._layers:
+            raise ValueError("accept needs a cache that holds the block")
+        B, block = self._batch_size(), int(block)
+        paths = check_paths(paths, B, block)
+        if any(l.seq_len < block for l in self._layers.values()):
+            raise ValueError(f"a layer holds fewer than {block} tokens")
+        counts = [len(p) for p in paths]
+        place = path_index(paths)
+        for layer in self._layers.values():
+            dev = layer.k_packed.device
+            base = layer.seq_len - block if layer.seq_lens is None else layer.seq_lens - block
+            if place is not None:
+                at = place.to(dev)
+                rows = at + (base if layer.seq_lens is None else base[:, None, None])
+                ops.move_rows((layer.k_packed, layer.k_scales, layer.v_packed, layer.v_scales),
+                              torch.where(at < 0, -1, rows).to(torch.int32), first=base)
+            longest = layer.seq_len - block + max(counts)
+            if layer.seq_lens is None and len(set(counts)) > 1:
+                lens = torch.tensor([base + c for c in counts], dtype=torch.int32)
+                layer.lag = _lag(lens, longest)
+                layer.seq_lens = lens.to(dev)
+            elif layer.seq_lens is not None:
+                # (in place: graphs and callers hold the tensor)
+                layer.seq_lens.copy_((base + torch.tensor(counts, dtype=torch.int32, device=dev)).clamp_(min=0))
+                layer.lag = None
+            layer.seq_len = longest
 
     def load_ragged(
         self,

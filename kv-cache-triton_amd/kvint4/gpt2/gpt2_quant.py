@@ -25,6 +25,7 @@ from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 from transformers.models.gpt2.modeling_gpt2 import GPT2Attention, eager_attention_forward
 
 from .attention_quant import attention_forward_quant
+from ..evicting import EvictingKVCache
 from ..module_swap import swap_attention_modules
 from ..paged_cache import PagedQuantizedKVCache
 from .kv_cache import QuantizedKVCache
@@ -71,6 +72,16 @@ class GPT2AttentionQuantized(GPT2Attention):
 
         using_eager = self.config._attn_implementation == "eager"
         fused_out = None
+        if isinstance(quant_cache, EvictingKVCache) and (attention_mask is not None or (using_eager and self.reorder_and_upcast_attn)):
+            raise ValueError("a cache that evicts takes no attention mask (padding, or a chunk after cached tokens) and "
+                             "no upcast attention")
+        if quant_cache.active_tree is not None:
+            # a tree of drafts: its mask stands for any other
+            quant_cache.append(key_states, value_states, self.layer_idx)
+            attn_output = quant_cache.attend_tree(query_states, self.layer_idx, quant_cache.active_tree,
+                                                  n_kv_heads=query_states.shape[1], scale=self.scaling).transpose(1, 2)
+            attn_output = attn_output.reshape(*attn_output.shape[:-2], -1).contiguous()
+            return self.resid_dropout(self.c_proj(attn_output)), None
         if attention_mask is None and query_states.shape[-2] == 1 and not (using_eager and self.reorder_and_upcast_attn):
             # decode token: append + attention in one launch (16-bit models)
             fused_out = quant_cache.append_and_attend(
@@ -88,7 +99,7 @@ class GPT2AttentionQuantized(GPT2Attention):
             attn_output, attn_weights = self._upcast_and_reordered_attn(
                 query_states, k_full.to(query_states.dtype), v_full.to(query_states.dtype), attention_mask
             )
-        elif attention_mask is None and isinstance(quant_cache, PagedQuantizedKVCache):
+        elif attention_mask is None and isinstance(quant_cache, (PagedQuantizedKVCache, EvictingKVCache)):
             attn_output = quant_cache.attend(
                 query_states, self.layer_idx, n_kv_heads=query_states.shape[1], scale=self.scaling,
                 is_causal=query_states.shape[-2] > 1,

@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from ..cache_base import QuantizedKVCacheBase, _LayerQuantizedKV  # noqa: F401  (re-export)
+from ..evicting import EvictingKVCache
 
 
 class QuantizedKVCache(QuantizedKVCacheBase):
@@ -47,3 +48,8 @@ class QuantizedKVCache(QuantizedKVCacheBase):
 
     def get_dequantized(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor]:
         return self._dequantized(layer_idx, torch.float16)
+
+
+class EvictingQuantizedKVCache(EvictingKVCache, QuantizedKVCache):
+    """QuantizedKVCache that keeps `budget` rows per head: the sinks, the recent
+    ones and those that drew most attention (kvint4.evicting)."""

@@ -17,6 +17,7 @@ from __future__ import annotations
 import torch
 
 from ..cache_base import QuantizedKVCacheBase, _LayerQuantizedKV  # noqa: F401  (re-export)
+from ..evicting import EvictingKVCache
 
 
 class QuantizedKVCache(QuantizedKVCacheBase):
@@ -60,3 +61,8 @@ class QuantizedKVCache(QuantizedKVCacheBase):
         out_dtype: torch.dtype = torch.bfloat16,
     ) -> tuple[torch.Tensor, torch.Tensor]:
         return self._dequantized(layer_idx, out_dtype)
+
+
+class EvictingQuantizedKVCache(EvictingKVCache, QuantizedKVCache):
+    """QuantizedKVCache that keeps `budget` rows per KV head: the sinks, the
+    recent ones and those that drew most attention (kvint4.evicting)."""

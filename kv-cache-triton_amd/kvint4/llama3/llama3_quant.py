@@ -12,6 +12,7 @@ Drop-in for ``models/llama3/llama3_quant.py`` (:36-204):
                     rows per KV head take the fused split-K kernel, prompts and
                     long chunks the matrix-core prefill kernel
         mask     -> dequantize the cache, HF attention interface with the mask
+        a tree of drafts is active (cache.tree) -> its own mask, attend_tree
     else: the stock path (cache.update + HF attention interface)
     -> o_proj
 
@@ -36,6 +37,7 @@ from transformers.models.llama.modeling_llama import (
 )
 
 from .attention_quant import attention_forward_quant_gqa
+from ..evicting import EvictingKVCache
 from ..module_swap import swap_attention_modules
 from ..paged_cache import PagedQuantizedKVCache
 from .kv_cache import QuantizedKVCache
@@ -70,6 +72,15 @@ class LlamaAttentionQuantized(LlamaAttention):
 
         if isinstance(past_key_values, (QuantizedKVCache, PagedQuantizedKVCache)):
             cache = past_key_values
+            if attention_mask is not None and isinstance(cache, EvictingKVCache):
+                raise ValueError("a cache that evicts takes no attention mask (padding, or a chunk after cached tokens)")
+            if cache.active_tree is not None:
+                # a tree of drafts: its mask stands for any other
+                cache.append(key_states, value_states, self.layer_idx)
+                attn_output = cache.attend_tree(query_states, self.layer_idx, cache.active_tree,
+                                                n_kv_heads=self.config.num_key_value_heads, scale=self.scaling)
+                attn_output = attn_output.transpose(1, 2).reshape(*input_shape, -1).contiguous()
+                return self.o_proj(attn_output), None
             if attention_mask is None and query_states.shape[-2] == 1:
                 # decode: append + attention in one launch
                 attn_output = cache.append_and_attend(
@@ -80,7 +91,7 @@ class LlamaAttentionQuantized(LlamaAttention):
                     attn_output = attn_output.transpose(1, 2).reshape(*input_shape, -1).contiguous()
                     return self.o_proj(attn_output), None
             cache.append(key_states, value_states, self.layer_idx)
-            if attention_mask is None and isinstance(cache, PagedQuantizedKVCache):
+            if attention_mask is None and isinstance(cache, (PagedQuantizedKVCache, EvictingKVCache)):
                 attn_output = cache.attend(
                     query_states, self.layer_idx, n_kv_heads=self.config.num_key_value_heads,
                     scale=self.scaling, is_causal=query_states.shape[-2] > 1,

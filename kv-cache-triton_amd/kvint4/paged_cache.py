@@ -39,9 +39,10 @@ from typing import Optional
 import torch
 
 from . import _native, ops
+from .tree_drafts import TreeDrafts, check_paths, path_index
 
 
-class PagedQuantizedKVCache:
+class PagedQuantizedKVCache(TreeDrafts):
     """INT4 KV cache in fixed-size pages.
 
     group_size: quantization group along d_head (as QuantizedKVCache).
@@ -387,6 +388,53 @@ class PagedQuantizedKVCache:
         return ops.dense_attention(query_states, k, v, n_kv_heads=n_kv_heads, is_causal=is_causal,
                                    sm_scale=scale, seq_lens=None if uniform else seq_lens)
 
+    # -- trees of drafted tokens -----------------------------------------------
+    def attend_tree(self, query_states: torch.Tensor, layer_idx: int, tree_mask: torch.Tensor, *, n_kv_heads: int,
+                    scale: float) -> torch.Tensor:
+        """Attention of a tree of T drafts, query_states [B, H_q, T, d], whose
+        rows are the last T of each sequence (appended before the call)."""
+        return ops.tree_attention_paged(
+            query_states, *self._pools[layer_idx], self._page_table(), tree_mask, n_kv_heads=n_kv_heads,
+            group_size=self.group_size, sm_scale=scale, seq_lens=self._seq_lens[layer_idx])
+
+    def accept(self, block: int, paths) -> None:
+        """Of the last `block` tokens of each sequence, in every layer, keep the
+        accepted ones: paths[b], ascending places in the block (none: an empty
+        list). Their rows move to the front of the block, the others are
+        dropped, and blocks past the new ends are released."""
+        if self._shape is None:
+            raise ValueError("accept needs a cache that holds the block")
+        B, block = self._shape[0], int(block)
+        paths = check_paths(paths, B, block)
+        if any(n < block for lens in self._lens.values() for n in lens):
+            raise ValueError(f"a sequence holds fewer than {block} tokens")
+        place = path_index(paths)
+        starts = {i: [n - block for n in lens] for i, lens in self._lens.items()}
+        if place is not None:
+            for lo in starts.values():  # (a block's rows are the sequence's own before any of them is written)
+                self._make_writable(lo, [len(p) for p in paths])
+            pt = self._page_table()
+            for i, lo in starts.items():
+                base = torch.tensor(lo, dtype=torch.int32)
+                rows = torch.where(place < 0, -1, place + base[:, None, None])
+                ops.move_rows_paged(self._pools[i], pt, rows.to(self._shape[5]), first=base.to(self._shape[5]))
+        for i, lo in starts.items():
+            self._set_lens(i, [n + len(p) for n, p in zip(lo, paths)])
+        self._release_past_ends()
+
+    def _set_lens(self, layer_idx: int, lens: list[int]) -> None:
+        self._lens[layer_idx] = lens
+        self._seq_lens[layer_idx].copy_(torch.tensor(lens, dtype=torch.int32))
+
+    def _release_past_ends(self) -> None:
+        """Release the blocks past every layer's end."""
+        P = self.page_size
+        for b, pages in enumerate(self._pages):
+            keep = -(-max((lens[b] for lens in self._lens.values()), default=0) // P)
+            while len(pages) > keep:
+                self._release(pages.pop())
+                self._table_dirty = True
+
     # -- batch and length edits (generate(): beam search, assisted decoding) --
     def _remap(self, src: list[int]) -> None:
         """New sequence b continues old sequence src[b] (sharing its blocks)."""
@@ -443,15 +491,8 @@ class PagedQuantizedKVCache:
         if max_length == 0 or self._shape is None:
             return
         for idx, lens in self._lens.items():
-            new = [max(n + max_length, 0) if max_length < 0 else min(n, max_length) for n in lens]
-            self._lens[idx] = new
-            self._seq_lens[idx].copy_(torch.tensor(new, dtype=torch.int32))
-        P = self.page_size
-        for b, pages in enumerate(self._pages):
-            keep = -(-max((lens[b] for lens in self._lens.values()), default=0) // P)
-            while len(pages) > keep:
-                self._release(pages.pop())
-                self._table_dirty = True
+            self._set_lens(idx, [max(n + max_length, 0) if max_length < 0 else min(n, max_length) for n in lens])
+        self._release_past_ends()
 
     # -- views ---------------------------------------------------------------
     def block_table(self) -> torch.Tensor:

@@ -31,6 +31,7 @@ from safetensors.torch import load_file, save_file
 
 from . import ops
 from .cache_base import QuantizedKVCacheBase, _lag, _LayerQuantizedKV
+from .evicting import EvictingKVCache
 from .paged_cache import PagedQuantizedKVCache
 
 FORMAT = "kvint4-cache"
@@ -48,6 +49,8 @@ def _layers_of(cache: Cache) -> list[int]:
 
 def save_cache(cache: Cache, path: str) -> None:
     """Write every layer of `cache` (layers 0 .. n-1, all present) to `path`."""
+    if isinstance(cache, EvictingKVCache):
+        raise ValueError("a cache that evicts cannot be saved: the format holds no positions, weights or tokens seen")
     idx = _layers_of(cache)
     if idx != list(range(len(idx))):
         raise ValueError(f"layers must be 0 .. n-1 (got {idx})")
@@ -107,6 +110,8 @@ def load_cache(path: str, cache: Cache, device: Union[str, torch.device] = "cuda
     meta, layers = read_cache_file(path)
     if int(meta["group_size"]) != cache.group_size:
         raise ValueError(f"file group size {meta['group_size']} != cache group size {cache.group_size}")
+    if isinstance(cache, EvictingKVCache):
+        raise ValueError("a cache that evicts cannot be loaded: the file holds no weights to rank its rows by")
     if _layers_of(cache):
         raise ValueError("load_cache needs an empty cache")
     dev = torch.device(device)
