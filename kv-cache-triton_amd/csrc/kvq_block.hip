@@ -683,6 +683,12 @@ __global__ __launch_bounds__(256) void block_finish_kernel(const BlockMfmaArgs a
   if (on) *w = before + sum;
 }
 
+template <int D, bool QF16>
+void launch_merge(const BlockMfmaArgs& a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.n_units * a.b.ratio * a.b.T;
+  hipLaunchKernelGGL((block_merge_kernel<D, QF16>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, st, a);
+}
+
 template <int D, bool QF16, int RB, int NW, bool SCORES>
 void launch_block(const BlockMfmaArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.n_units * a.row_chunks * a.n_split)), block(64 * NW);
@@ -691,11 +697,7 @@ void launch_block(const BlockMfmaArgs& a, hipStream_t st) {
   } else {
     hipLaunchKernelGGL((block_attn_kernel<D, QF16, RB, NW, false, SCORES>), grid, block, 0, st, a);
   }
-  if (a.n_split > 1 && !SCORES) {
-    const int64_t rows = (int64_t)a.n_units * a.b.ratio * a.b.T;
-    hipLaunchKernelGGL((block_merge_kernel<D, QF16>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0,
-                       st, a);
-  }
+  if (a.n_split > 1 && !SCORES) launch_merge<D, QF16>(a, st);
 }
 
 template <int D, bool QF16>
@@ -766,14 +768,16 @@ bool block_mfma_takes(const BlockArgs& a) {
          dense_rows(a.vs, a.vss_b, a.vss_h, a.vss_s, a.D / a.G, a.D / a.G, 2);
 }
 
-namespace {
+void launch_block_merge(const BlockMfmaArgs& a, hipStream_t st) {
+  const bool f16 = a.b.q_dt == KVQ_F16;
+  if (a.b.D == 128) f16 ? launch_merge<128, true>(a, st) : launch_merge<128, false>(a, st);
+  else f16 ? launch_merge<64, true>(a, st) : launch_merge<64, false>(a, st);
+}
 
-void fill_mfma(BlockMfmaArgs* a, const BlockArgs& b, const BlockPlan& p) {
+void fill_block_mfma(BlockMfmaArgs* a, const BlockArgs& b) {
   *a = BlockMfmaArgs{};
   a->b = b;
   a->n_units = b.B * b.Hkv;
-  a->row_chunks = (int)p.row_chunks;
-  a->n_split = (int)p.n_split;
   a->ng = b.D / b.G;
   a->s_f16 = b.s_dt == KVQ_F16;
   a->tiles_max = (int)((b.Sk + kKeys - 1) / kKeys);
@@ -783,6 +787,8 @@ void fill_mfma(BlockMfmaArgs* a, const BlockArgs& b, const BlockPlan& p) {
   a->q_vec = mult(b.q, 16, b.qs_b, b.qs_h, b.qs_s, 8);
   a->o_vec = b.out && mult(b.out, 8, b.os_b, b.os_h, b.os_s, 4);
 }
+
+namespace {
 
 int launch_any(const BlockMfmaArgs& a, const BlockPlan& p, hipStream_t st) {
   if ((int64_t)a.n_units * a.row_chunks * a.n_split >= (int64_t(1) << 31)) return KVQ_EUNSUP;
@@ -799,11 +805,33 @@ int launch_any(const BlockMfmaArgs& a, const BlockPlan& p, hipStream_t st) {
 
 }  // namespace
 
-int launch_block_mfma(const BlockArgs& b, BlockPlan p, void* workspace, int64_t workspace_bytes, hipStream_t st) {
-  if (p.n_split > 1 && (workspace == nullptr || workspace_bytes < p.ml_bytes + p.o_bytes || (uintptr_t)workspace % 16 != 0))
-    p.n_split = 1;
+int64_t block_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk) {
+  if (T * (Hq / Hkv) > kRowsMin) {
+    const RowsPlan p = rows_plan(B, Hq, Hkv, T, D, Sk, false);
+    return p.ml_bytes + p.o_bytes;
+  }
+  const BlockPlan p = block_plan(B, Hq, Hkv, T, D, Sk);
+  return p.ml_bytes + p.o_bytes;
+}
+
+int launch_block_mfma(const BlockArgs& b, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+  const bool fits = workspace != nullptr && (uintptr_t)workspace % 16 == 0 &&
+                    workspace_bytes >= block_workspace_bytes(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk);
+  if ((int64_t)b.T * b.ratio > kRowsMin) {
+    RowsPlan p = rows_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk, false);
+    if (!fits) p.n_split = 1;
+    RowsArgs a = {};
+    fill_block_mfma(&a.m, b);
+    a.m.ws_ml = (float2*)workspace;
+    a.m.ws_o = (float*)((char*)workspace + p.ml_bytes);
+    return launch_rows(a, p, false, st);
+  }
+  BlockPlan p = block_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk);
+  if (!fits) p.n_split = 1;
   BlockMfmaArgs a;
-  fill_mfma(&a, b, p);
+  fill_block_mfma(&a, b);
+  a.row_chunks = (int)p.row_chunks;
+  a.n_split = (int)p.n_split;
   a.ws_ml = (float2*)workspace;
   a.ws_o = (float*)((char*)workspace + p.ml_bytes);
   return launch_any(a, p, st);
@@ -821,7 +849,9 @@ int launch_block_weights(const BlockArgs& b, float* weights, const int64_t* ws, 
   const int64_t rows = (int64_t)b.ratio * b.T;
   const BlockPlan p = block_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk);
   BlockMfmaArgs a;
-  fill_mfma(&a, b, p);
+  fill_block_mfma(&a, b);
+  a.row_chunks = (int)p.row_chunks;
+  a.n_split = (int)p.n_split;
   const int64_t ml = ((int64_t)a.n_units * rows * p.n_split * 8 + 255) / 256 * 256;
   a.ws_ml = (float2*)workspace;
   a.ws_o = (float*)((char*)workspace + ml);

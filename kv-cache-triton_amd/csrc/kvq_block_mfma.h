@@ -34,13 +34,39 @@ BlockPlan block_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, i
 bool block_mfma_takes_keys(const BlockArgs& a);
 bool block_mfma_takes(const BlockArgs& a);
 
-// Without workspace for the plan's split the launch does not split.
-int launch_block_mfma(const BlockArgs& b, BlockPlan p, void* workspace, int64_t workspace_bytes, hipStream_t st);
+// Attention by the kernel of few rows or of many; without the workspace for its
+// split the launch does not split.
+int64_t block_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk);
+int launch_block_mfma(const BlockArgs& b, void* workspace, int64_t workspace_bytes, hipStream_t st);
 
 // Attention that keeps its scores, and the key weights from them, for up to
 // kMaxScoreRows rows per KV head; workspace bytes (0 for more rows).
 int64_t block_scores_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk);
 int launch_block_weights(const BlockArgs& b, float* weights, const int64_t* ws, void* workspace, hipStream_t st);
+
+// Merges the splits' partials of a launch that leaves them in ws_ml and ws_o.
+void launch_block_merge(const BlockMfmaArgs& a, hipStream_t st);
+void fill_block_mfma(BlockMfmaArgs* a, const BlockArgs& b);
+
+// Many rows per KV head (kvq_rows.hip): the arguments of the kernel, with the
+// row's units and query operands to keep for the key weights' second pass (or
+// null), its plan and launch.
+struct RowsArgs {
+  BlockMfmaArgs m;
+  float* row_unit;  // [unit][row]
+  uint4* q_img;     // [unit][32-row block][16-dim step][64]
+  int* q_odd;       // [unit][32-row block]: a query is not finite
+  int q_blocks;
+};
+
+struct RowsPlan {
+  int nw;
+  int64_t row_chunks, n_split, ml_bytes, o_bytes;
+};
+
+constexpr int64_t kRowsMin = 32;  // more rows per KV head than this take it
+RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool two);
+int launch_rows(RowsArgs a, const RowsPlan& p, bool two, hipStream_t st);
 
 // Key weights of blocks of any length (kvq_sums.hip), for what
 // block_mfma_takes_keys takes of a contiguous cache.

@@ -11,34 +11,21 @@
 //                      stay in registers, query tiles go through LDS
 //   key_add_kernel     the shares' sums to the running sums, in a fixed order
 //
-// Scores are exact to fp32's rounding: a key's scales and a row's queries are
-// brought near 1 by powers of two of their own (taken back in fp32 after the
-// product), and then
-//   - a bf16 query fits fp16;
-//   - a code times a bf16 scale has 3 + 8 significant bits and fits fp16 too (a
-//     group whose scale is under 2^-14 of the key's largest is off by 2^-25 of
-//     that, fp32's own rounding of the sum);
-//   - a code times an fp16 scale has 14 bits: TWO keeps it as fp16 hi + lo, and
-//     takes both products.
+// Scores are exact to fp32's rounding (kvq_operands.h).
 // Both passes form them by the same instructions in the same order, so that a
 // row's weights add up to 1.
 //
 // Layout of the 32x32x16 instruction (lane l: n = l % 32, g = l / 32): A[i][k] and
 // B[k][n] at lane (i or n, k / 8), register k % 8; C[r][n] at lane n + 32 ((r / 4)
 // % 2), register 4 (r / 8) + r % 4. A lane holds, of query row n, keys 8 (r / 4) +
-// 4 g + r % 4. The eight dims of an operand piece are in the order (0, 4), (1, 5),
-// (2, 6), (3, 7) of pairs, which the nibbles of a code word give for free.
+// 4 g + r % 4.
 
 #include <algorithm>
 
-#include "kvq_block_mfma.h"
+#include "kvq_operands.h"
 
 namespace kvq {
 namespace {
-
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 64;  // keys of a tile of the first pass, rows of one of the second
 constexpr float kNeg = -1.0e30f;
@@ -59,102 +46,6 @@ struct SumArgs {
   float* weights;
   int64_t w_b, w_h, w_k;
 };
-
-__device__ __forceinline__ f32x16_t mfma(uint4 a, uint4 b, f32x16_t c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ float pair_max(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-  const uint32_t r0 = r[0], r1 = r[1];
-  return fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
-}
-__device__ __forceinline__ float pair_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-  const uint32_t r0 = r[0], r1 = r[1];
-  return __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
-}
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
-  uint32_t d;
-  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(d) : "v"(x), "s"(m), "v"(o));
-  return d;
-}
-__device__ __forceinline__ uint32_t u32_of(f16x2_t v) { return __builtin_bit_cast(uint32_t, v); }
-
-// The power of two that takes x > 0 into [1, 2), between 2^-100 and 2^100 (1 for 0).
-__device__ __forceinline__ float unit_of(float x) {
-  if (!(x > 0.0f)) return 1.0f;
-  const int e = 127 - (int)(__builtin_bit_cast(uint32_t, x) >> 23);
-  const int u = e < -100 ? -100 : (e > 100 ? 100 : e);
-  return __builtin_bit_cast(float, (uint32_t)(u + 127) << 23);
-}
-
-// The eight codes of w times the scale s, as fp16 (TWO: the rest of the product
-// as fp16 in lo).
-template <bool TWO>
-__device__ __forceinline__ uint4 decode(uint32_t w, _Float16 s, uint4* lo) {
-  const f16x2_t ss = {s, s}, off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-  uint32_t hi[4], rest[4];
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const f16x2_t n = __builtin_bit_cast(f16x2_t, and_or(w >> (4 * p), 0x000f000fu, 0x64006400u)) + off;
-    const f16x2_t v = n * ss;
-    hi[p] = u32_of(v);
-    if constexpr (TWO) rest[p] = u32_of(__builtin_elementwise_fma(n, ss, -v));
-  }
-  if constexpr (TWO) *lo = make_uint4(rest[0], rest[1], rest[2], rest[3]);
-  return make_uint4(hi[0], hi[1], hi[2], hi[3]);
-}
-
-// A key's scale row (up to four 16-bit scales in x): scale c as fp32.
-__device__ __forceinline__ float scale_at(uint64_t x, int c, int s_f16) {
-  const uint32_t v = (uint32_t)(x >> (16 * c)) & 0xffffu;
-  return s_f16 ? f16_bits_to_f32(v) : bf16_bits_to_f32(v);
-}
-__device__ __forceinline__ uint64_t load_scale_row(const uint16_t* p, int ng) {
-  if (ng == 4) {
-    const uint2 v = *(const uint2*)p;
-    return ((uint64_t)v.y << 32) | v.x;
-  }
-  return ng == 2 ? *(const uint32_t*)p : *p;
-}
-// The power of two of a key's scales, and whether one is not finite.
-__device__ __forceinline__ float key_unit(uint64_t x, int ng, int s_f16, bool* odd) {
-  float top = 0.0f;
-  for (int c = 0; c < ng; ++c) {
-    const float v = fabsf(scale_at(x, c, s_f16));
-    if (v < __builtin_inff()) top = fmaxf(top, v);
-    else *odd = true;
-  }
-  return unit_of(top);
-}
-
-// Eight query elements, as fp32 and as an operand piece times `unit`.
-template <bool QF16>
-__device__ __forceinline__ void query_floats(uint4 x, float (&f)[8]) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    f[2 * k] = QF16 ? f16_bits_to_f32(w[k] & 0xffffu) : bf16_bits_to_f32(w[k] & 0xffffu);
-    f[2 * k + 1] = QF16 ? f16_bits_to_f32(w[k] >> 16) : bf16_bits_to_f32(w[k] >> 16);
-  }
-}
-template <bool QF16>
-__device__ __forceinline__ uint4 query_piece(uint4 x, float unit) {
-  float f[8];
-  query_floats<QF16>(x, f);
-  uint32_t p[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const f16x2_t v = {(_Float16)(f[k] * unit), (_Float16)(f[k + 4] * unit)};
-    p[k] = u32_of(v);
-  }
-  return make_uint4(p[0], p[1], p[2], p[3]);
-}
-__device__ __forceinline__ uint4 load_query(const uint16_t* p, bool vec) {
-  if (vec) return *(const uint4*)p;
-  return make_uint4((uint32_t)p[0] | ((uint32_t)p[1] << 16), (uint32_t)p[2] | ((uint32_t)p[3] << 16),
-                    (uint32_t)p[4] | ((uint32_t)p[5] << 16), (uint32_t)p[6] | ((uint32_t)p[7] << 16));
-}
 
 // Keys that row R may attend: [0, limit).
 __device__ __forceinline__ int row_limit(const SumArgs& a, int R, int len) {

@@ -336,7 +336,7 @@ int tree_impl(const char* what, const void* q, int q_dtype, const int64_t* q_str
   a.out = out;
   a.os_b = out_strides[0]; a.os_h = out_strides[1]; a.os_s = out_strides[2]; a.os_d = out_strides[3];
   if (block_mfma_takes(a)) {
-    const int lc = launch_block_mfma(a, block_plan(B, Hq, Hkv, T, D, Sk), workspace, workspace_bytes, (hipStream_t)stream);
+    const int lc = launch_block_mfma(a, workspace, workspace_bytes, (hipStream_t)stream);
     KVQ_CHECK_ARG(lc == KVQ_OK, "%s: too large", what);
   } else {
     launch_block_rows(a, (hipStream_t)stream);
@@ -383,6 +383,5 @@ extern "C" int64_t kvq_tree_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t 
     return KVQ_EINVAL;
   }
   if (B == 0 || T == 0 || !(D == 64 || D == 128) || q_dtype == KVQ_F32 || scale_dtype == KVQ_F32) return 0;
-  const BlockPlan p = block_plan(B, Hq, Hkv, T, D, Sk);
-  return p.ml_bytes + p.o_bytes;
+  return block_workspace_bytes(B, Hq, Hkv, T, D, Sk);
 }

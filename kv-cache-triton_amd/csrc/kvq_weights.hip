@@ -89,10 +89,7 @@ int64_t workspace_needed(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t 
   if (B == 0 || T == 0 || !(D == 64 || D == 128) || q_dt == KVQ_F32 || s_dt == KVQ_F32) return n;
   if (with_out && takes_scores(B, Hq, Hkv, T, D, Sk, q_dt, s_dt)) return std::max(n, block_scores_bytes(B, Hq, Hkv, T, D, Sk));
   n = std::max(n, sums_workspace_bytes(B, Hq, Hkv, T, Sk, s_dt == KVQ_F16));
-  if (with_out) {
-    const BlockPlan p = block_plan(B, Hq, Hkv, T, D, Sk);
-    n = std::max(n, p.ml_bytes + p.o_bytes);
-  }
+  if (with_out) n = std::max(n, block_workspace_bytes(B, Hq, Hkv, T, D, Sk));
   return n;
 }
 
@@ -137,7 +134,7 @@ int weights_impl(const char* what, const void* q, int q_dtype, const int64_t* q_
     a.stats = nullptr;
     if (a.out) {
       if (block_mfma_takes(a)) {
-        const int lc = launch_block_mfma(a, block_plan(B, Hq, Hkv, T, D, Sk), workspace, workspace_bytes, st);
+        const int lc = launch_block_mfma(a, workspace, workspace_bytes, st);
         KVQ_CHECK_ARG(lc == KVQ_OK, "%s: too large", what);
       } else {
         launch_block_rows(a, st);

@@ -21,7 +21,7 @@ CSRC = os.path.join(PKG_ROOT, "csrc")
 OUT = os.path.join(_HERE, "libkvint4.so")
 
 SOURCES = ("kvq_capi.hip", "kvq_quant.hip", "kvq_attn.hip", "kvq_prefill.hip", "kvq_tree.hip", "kvq_block.hip",
-           "kvq_weights.hip", "kvq_sums.hip", "kvq_evict.hip")
+           "kvq_rows.hip", "kvq_weights.hip", "kvq_sums.hip", "kvq_evict.hip")
 # Per-source flags. The decode kernels keep their MFMA accumulators in VGPRs:
 # the compiler's default puts the PV accumulators in AGPRs, and the two-row-set
 # kernel then copies about 72 values between AGPRs and VGPRs on every tile
@@ -30,7 +30,8 @@ SOURCES = ("kvq_capi.hip", "kvq_quant.hip", "kvq_attn.hip", "kvq_prefill.hip", "
 # (176 copies) and runs four waves per SIMD instead of three.
 SOURCE_FLAGS = {"kvq_attn.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true"),
                 "kvq_prefill.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true"),
-                "kvq_block.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true")}
+                "kvq_block.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true"),
+                "kvq_rows.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true")}
 # gfx950 only: the decode kernels assume its wave64 MFMA forms and its
 # round-robin workgroup-to-XCD dispatch (checked again at run time).
 ARCH = "gfx950"
