@@ -31,7 +31,7 @@ struct BlockArgs {
   int64_t ms_b, ms_i, ms_t;
   void* out;
   int64_t os_b, os_h, os_s, os_d;
-  // [B, Hq, T] (m, 1 / l) of each row, weight j = 2^(s_j - m) / l, or null. A row
+  // [B, Hkv, row] (m, 1 / l) of each row, weight j = 2^(s_j - m) / l, or null. A row
   // with no key has 1 / l = 0. The pair, not m + log2 l: at
   // scores in the thousands the sum's rounding alone is 2^-12 of a weight.
   float2* stats;
@@ -41,6 +41,11 @@ struct BlockArgs {
   int B, Hq, Hkv, ratio, T, D, G;
   float scale_log2;  // sm_scale * log2(e)
 };
+
+// Where `stats` has query row i of head h: row i * ratio + h % ratio of the KV head.
+__device__ __forceinline__ int64_t stats_at(const BlockArgs& a, int b, int h, int i) {
+  return ((int64_t)b * a.Hkv + h / a.ratio) * a.ratio * a.T + (int64_t)i * a.ratio + h % a.ratio;
+}
 
 // Keys of sequence b: its device length clamped to [0, Sk], or Sk.
 __device__ __forceinline__ int64_t block_len(const BlockArgs& a, int b) {

@@ -824,7 +824,7 @@ int launch_block_mfma(const BlockArgs& b, void* workspace, int64_t workspace_byt
     fill_block_mfma(&a.m, b);
     a.m.ws_ml = (float2*)workspace;
     a.m.ws_o = (float*)((char*)workspace + p.ml_bytes);
-    return launch_rows(a, p, false, st);
+    return launch_rows(a, p, st);
   }
   BlockPlan p = block_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk);
   if (!fits) p.n_split = 1;

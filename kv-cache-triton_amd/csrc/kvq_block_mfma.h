@@ -48,15 +48,20 @@ int launch_block_weights(const BlockArgs& b, float* weights, const int64_t* ws, 
 void launch_block_merge(const BlockMfmaArgs& a, hipStream_t st);
 void fill_block_mfma(BlockMfmaArgs* a, const BlockArgs& b);
 
-// Many rows per KV head (kvq_rows.hip): the arguments of the kernel, with the
-// row's units and query operands to keep for the key weights' second pass (or
-// null), its plan and launch.
+// The queries as matrix operands, kept for the key weights' second pass.
+struct QueryImages {
+  float* unit;  // [unit][row]: the power of two of the row
+  uint4* img;   // [unit][32-row block][16-dim step][64]
+  int* odd;     // [unit][32-row block]: a query is not finite
+  int blocks;
+};
+
+// Many rows per KV head (kvq_rows.hip): the arguments of the kernel, its plan
+// and launch. With qi.img it keeps the query operands and sums the softmax in
+// full precision; `two`: such a launch on fp16 scales.
 struct RowsArgs {
   BlockMfmaArgs m;
-  float* row_unit;  // [unit][row]
-  uint4* q_img;     // [unit][32-row block][16-dim step][64]
-  int* q_odd;       // [unit][32-row block]: a query is not finite
-  int q_blocks;
+  QueryImages qi;
 };
 
 struct RowsPlan {
@@ -65,13 +70,14 @@ struct RowsPlan {
 };
 
 constexpr int64_t kRowsMin = 32;  // more rows per KV head than this take it
-RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool two);
-int launch_rows(RowsArgs a, const RowsPlan& p, bool two, hipStream_t st);
+RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool weights);
+int launch_rows(RowsArgs a, const RowsPlan& p, hipStream_t st);
 
 // Key weights of blocks of any length (kvq_sums.hip), for what
 // block_mfma_takes_keys takes of a contiguous cache.
-int64_t sums_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t Sk, bool s_f16);
-int launch_key_sums(const BlockArgs& b, float* weights, const int64_t* ws, void* workspace, hipStream_t st);
+// With `attend` the block's attention too, whose statistics the sums then take.
+int64_t sums_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool s_f16, bool attend);
+int launch_key_sums(const BlockArgs& b, bool attend, float* weights, const int64_t* ws, void* workspace, hipStream_t st);
 
 // Dims d .. d + 3 of output row R (row R / ratio of the block, head R % ratio
 // of the group), and the row's statistics, from a row's max, sum and
@@ -81,7 +87,7 @@ __device__ __forceinline__ void block_store_row(const BlockMfmaArgs& a, int b, i
                                                 float4 o) {
   const int i = R / a.b.ratio, h = kvh * a.b.ratio + R % a.b.ratio;
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  if (a.b.stats && d == 0) a.b.stats[((int64_t)b * a.b.Hq + h) * a.b.T + i] = make_float2(m, inv);
+  if (a.b.stats && d == 0) a.b.stats[((int64_t)b * a.b.Hkv + kvh) * a.b.ratio * a.b.T + R] = make_float2(m, inv);
   if (!a.b.out) return;
   uint16_t* p = (uint16_t*)a.b.out + b * a.b.os_b + (int64_t)h * a.b.os_h + (int64_t)i * a.b.os_s + d;
   const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};

@@ -39,9 +39,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* p, uint32_
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
 }
 
-template <int D, bool QF16, bool SF16, bool TWO, int NW, bool PAGED>
+// SUMS: for key weights: the sums of the softmax in fp32 (as the products take
+// them, else), the query operands kept, and both terms of fp16 scales (TWO).
+template <int D, bool QF16, bool SF16, bool SUMS, int NW, bool PAGED>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void rows_attn_kernel(const RowsArgs a) {
+  constexpr bool TWO = SUMS && SF16;
   constexpr int NT = 64 * NW, ROWS = 32 * NW;
   constexpr int KS = D / 16;           // 16-dim steps of S^T
   constexpr int NDB = D / 32;          // 32-dim blocks of O^T
@@ -84,6 +87,13 @@ void rows_attn_kernel(const RowsArgs a) {
     const uint16_t* p = (const uint16_t*)ab.q + b * ab.qs_b + (int64_t)head * ab.qs_h + (int64_t)row_i * ab.qs_s + 8 * g;
     q_unit = query_operand<QF16, KS>(p, a.m.q_vec, ab.scale_log2 < 0.0f, q, &q_odd);
     q_odd = __builtin_amdgcn_ballot_w64(q_odd) != 0;
+    if (SUMS && sp == 0 && R0 < rows) {
+      const int64_t block = (int64_t)unit * a.qi.blocks + R0 / 32;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) a.qi.img[(block * KS + kk) * 64 + lane] = q[kk];
+      if (lane == 0) a.qi.odd[block] = q_odd;
+      if (g == 0 && R < rows) a.qi.unit[(int64_t)unit * rows + R] = q_unit;
+    }
   }
 
   // ---- tiles: first cache row and rows of tile t ----
@@ -339,20 +349,20 @@ void rows_attn_kernel(const RowsArgs a) {
       uint32_t seen = 0u;
       if (nr_cur > 0) {
         if (cb.kind == kMaskTree) {
-          // (clamped loads without conditions: eight in flight)
+          // (clamped loads without conditions: sixteen in flight)
           const uint8_t* mrow = cb.mask + b * cb.ms_b + (int64_t)row_i * cb.ms_i;
           const int64_t ms_t = cb.ms_t;
           const int T = cb.T;
 #pragma unroll 1
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < 2; ++x) {
             uint32_t on = 0u;
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              const int k = t0 + 16 * x + 8 * (y >> 2) + 4 * gc + (y & 3), t = k - base;
+            for (int y = 0; y < 16; ++y) {
+              const int k = t0 + 32 * x + 8 * (y >> 2) + 4 * gc + (y & 3), t = k - base;
               const uint8_t set = mrow[(int64_t)min(max(t, 0), T - 1) * ms_t];
               on |= k < len && (t < 0 || set != 0) ? 1u << y : 0u;
             }
-            seen |= on << (8 * x);
+            seen |= on << (16 * x);
           }
         } else {
           const int lim = limit(row_i);
@@ -399,10 +409,11 @@ void rows_attn_kernel(const RowsArgs a) {
         for (int w = 0; w < 16; ++w) {
           if (MAXES + 1 + w * (NM - MAXES - 1) / 16 != x) continue;
           const int kb = w >> 3, r = 2 * (w & 7);
-          const f16x2_t h = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], cr, -m_run)),
-                             (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r + 1], cr, -m_run))};
-          const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
-          ls = __builtin_amdgcn_fdot2(h, one, ls, false);  // the weights as the products take them
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], cr, -m_run));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r + 1], cr, -m_run));
+          const f16x2_t h = {(_Float16)e0, (_Float16)e1}, one = {(_Float16)1.0f, (_Float16)1.0f};
+          if constexpr (SUMS) ls += e0 + e1;
+          else ls = __builtin_amdgcn_fdot2(h, one, ls, false);
           ((uint32_t*)&pc[w >> 2])[w & 3] = u32_of(h);
         }
       }
@@ -507,45 +518,52 @@ void rows_attn_kernel(const RowsArgs a) {
     }
 }
 
-template <int D, bool QF16, bool SF16, bool TWO, int NW>
+template <int D, bool QF16, bool SF16, bool SUMS, int NW>
 void launch(const RowsArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)a.m.n_units, (unsigned)a.m.row_chunks, (unsigned)a.m.n_split), block(64 * NW);
-  if constexpr (!TWO)
+  if constexpr (!SUMS)
     if (a.m.b.pm.paged) {
-      hipLaunchKernelGGL((rows_attn_kernel<D, QF16, SF16, TWO, NW, true>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((rows_attn_kernel<D, QF16, SF16, SUMS, NW, true>), grid, block, 0, st, a);
       return;
     }
-  hipLaunchKernelGGL((rows_attn_kernel<D, QF16, SF16, TWO, NW, false>), grid, block, 0, st, a);
+  hipLaunchKernelGGL((rows_attn_kernel<D, QF16, SF16, SUMS, NW, false>), grid, block, 0, st, a);
 }
 
-template <int D, bool QF16>
-void launch_two(const RowsArgs& a, bool two, int nw, hipStream_t st) {
-  const bool f16 = a.m.s_f16;
-  if (two && f16) launch<D, QF16, true, true, 8>(a, st);
-  else if (nw == 8) f16 ? launch<D, QF16, true, false, 8>(a, st) : launch<D, QF16, false, false, 8>(a, st);
-  else f16 ? launch<D, QF16, true, false, 4>(a, st) : launch<D, QF16, false, false, 4>(a, st);
+template <int D, bool QF16, bool SF16>
+void launch_waves(const RowsArgs& a, int nw, hipStream_t st) {
+  if (a.qi.img) launch<D, QF16, SF16, true, 8>(a, st);
+  else if (nw == 8) launch<D, QF16, SF16, false, 8>(a, st);
+  else launch<D, QF16, SF16, false, 4>(a, st);
+}
+
+template <int D>
+void launch_types(const RowsArgs& a, int nw, hipStream_t st) {
+  const bool q16 = a.m.b.q_dt == KVQ_F16;
+  if (a.m.s_f16) q16 ? launch_waves<D, true, true>(a, nw, st) : launch_waves<D, false, true>(a, nw, st);
+  else q16 ? launch_waves<D, true, false>(a, nw, st) : launch_waves<D, false, false>(a, nw, st);
 }
 
 }  // namespace
 
-RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool two) {
+RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool weights) {
   const int64_t rows = T * (Hq / Hkv), units = B * Hkv, tiles = (Sk + kTile - 1) / kTile;
   RowsPlan p;
   // eight waves (256 rows, one workgroup per CU), or four, two workgroups per
-  // CU, where eight would leave four without rows; two terms take the LDS of
-  // eight waves' workgroup
-  p.nw = two || (rows + 127) / 128 % 2 == 0 || rows > 1024 ? 8 : 4;
+  // CU, where eight would leave four without rows; key weights are
+  // of prompts, with rows enough
+  p.nw = weights || (rows + 127) / 128 % 2 == 0 || rows > 1024 ? 8 : 4;
   p.row_chunks = (rows + 32 * p.nw - 1) / (32 * p.nw);
-  // the split with the least estimate: rounds of the workgroups that are
-  // resident together, each its tiles and about four tiles' time of prologue
-  // and epilogue; a merge costs its launch and the partials' traffic
+  // the split with the least estimate, in tiles' times (2.2 us): rounds of the
+  // workgroups that are resident together, each its tiles and about six tiles'
+  // time of prologue and epilogue; the partials' traffic (33 MB in 14 us) and a
+  // merge's launch
   const int64_t wgs = units * p.row_chunks, slots = p.nw == 8 ? 256 : 512;
   p.n_split = 1;
   double best = 0.0;
   for (int64_t ns = 1; ns <= std::min<int64_t>(64, std::max<int64_t>(1, tiles / 4)); ++ns) {
     const double rounds = (double)((wgs * ns + slots - 1) / slots);
-    const double cost = rounds * ((double)((tiles + ns - 1) / ns) + 4.0) +
-                        (ns > 1 ? 3.0 + (double)(units * rows * ns) * (double)D * 8.0 / 4.0e6 : 0.0);
+    const double cost = rounds * ((double)((tiles + ns - 1) / ns) + 6.0) +
+                        (ns > 1 ? 2.5 + (double)(units * rows * ns) * (double)D / 1.2e6 : 0.0);
     if (ns == 1 || cost < best) {
       best = cost;
       p.n_split = ns;
@@ -559,18 +577,12 @@ RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int
   return p;
 }
 
-int launch_rows(RowsArgs a, const RowsPlan& p, bool two, hipStream_t st) {
-  if (p.row_chunks >= 65536 || (int64_t)a.m.b.Sk >= (int64_t(1) << 31)) return KVQ_EUNSUP;
+int launch_rows(RowsArgs a, const RowsPlan& p, hipStream_t st) {
+  if (p.row_chunks >= 65536 || a.m.b.Sk >= (int64_t(1) << 31)) return KVQ_EUNSUP;
   a.m.row_chunks = (int)p.row_chunks;
   a.m.n_split = (int)p.n_split;
-  const bool f16 = a.m.b.q_dt == KVQ_F16;
-  if (a.m.b.D == 128) {
-    if (f16) launch_two<128, true>(a, two, p.nw, st);
-    else launch_two<128, false>(a, two, p.nw, st);
-  } else {
-    if (f16) launch_two<64, true>(a, two, p.nw, st);
-    else launch_two<64, false>(a, two, p.nw, st);
-  }
+  if (a.m.b.D == 128) launch_types<128>(a, p.nw, st);
+  else launch_types<64>(a, p.nw, st);
   if (p.n_split > 1) launch_block_merge(a.m, st);
   return KVQ_OK;
 }

@@ -3,17 +3,18 @@
 //
 // Two passes over the scores S^T = K Q^T (v_mfma 32x32x16, both operands fp16),
 // since a key's sum needs every row's softmax statistics first:
+//   the attention (kvq_rows.hip), or without values
 //   row_stats_kernel   (m, l) of each row over a share of the keys: the queries
 //                      stay in registers (64 rows a wave), key tiles are decoded
 //                      once per workgroup into an LDS image of the A operand
 //   row_merge_kernel   the shares' statistics to (m, 1 / l)
+// either of which also leaves the queries as fp16 operands, and
 //   key_sums_kernel    sum over a share of the rows of 2^(s - m) / l: the keys
 //                      stay in registers, query tiles go through LDS
 //   key_add_kernel     the shares' sums to the running sums, in a fixed order
 //
-// Scores are exact to fp32's rounding (kvq_operands.h).
-// Both passes form them by the same instructions in the same order, so that a
-// row's weights add up to 1.
+// Scores are exact to fp32's rounding (kvq_operands.h). Both passes form them by
+// the same instructions in the same order, so that a row's weights add up to 1.
 //
 // Layout of the 32x32x16 instruction (lane l: n = l % 32, g = l / 32): A[i][k] and
 // B[k][n] at lane (i or n, k / 8), register k % 8; C[r][n] at lane n + 32 ((r / 4)
@@ -36,11 +37,11 @@ constexpr int kSumRowTiles = 16; // row tiles of a share of the second pass
 
 struct SumArgs {
   BlockArgs b;
+  QueryImages qi;
   int n_units, ng, s_f16, q_vec;
   int row_blocks, splits;  // first pass: row blocks, shares of the keys
   int key_blocks, chunks;  // second pass: key blocks, shares of the rows
   float2* part;            // [unit][row][split] (m, l)
-  float* row_unit;         // [unit][row] power of two of the row's queries
   float2* stats;           // [unit][row] (m, 1 / l)
   float* sums;             // [unit][chunk][Sk]
   float* weights;
@@ -82,39 +83,29 @@ void row_stats_kernel(const SumArgs a) {
 
   // queries as the B operand, rows 32 r + n of the wave
   const float c = fmaxf(fabsf(a.b.scale_log2), 1.0e-30f);
-  const uint32_t qneg = a.b.scale_log2 < 0.0f ? 0x80008000u : 0u;
   uint4 q[2][KS];
   float cr[2];
   int lim[2];
   bool odd_q = false;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int R = blk * kStatRows + wave * 64 + 32 * r + n, Rc = R < rows ? R : rows - 1;
+    const int R0 = blk * kStatRows + wave * 64 + 32 * r, R = R0 + n, Rc = R < rows ? R : rows - 1;
     lim[r] = row_limit(a, R, len);
     const int i = Rc / a.b.ratio, h = kvh * a.b.ratio + Rc % a.b.ratio;
     const uint16_t* p = (const uint16_t*)a.b.q + b * a.b.qs_b + (int64_t)h * a.b.qs_h + (int64_t)i * a.b.qs_s + 8 * g;
-    float top = 0.0f;
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-      uint4 x = load_query(p + 16 * kk, a.q_vec);
-      x = make_uint4(x.x ^ qneg, x.y ^ qneg, x.z ^ qneg, x.w ^ qneg);
-      q[r][kk] = x;
-      float f[8];
-      query_floats<QF16>(x, f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float v = fabsf(f[k]);
-        if (v < __builtin_inff()) top = fmaxf(top, v);
-        else odd_q = true;
-      }
-    }
-    const float u = unit_of(pair_max(top));
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) q[r][kk] = query_piece<QF16>(q[r][kk], u);
+    bool odd = false;
+    const float u = query_operand<QF16, KS>(p, a.q_vec, a.b.scale_log2 < 0.0f, q[r], &odd);
+    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    odd_q = odd_q || odd;
     cr[r] = c / u;
-    if (sp == 0 && g == 0 && R < rows) a.row_unit[(int64_t)unit * rows + R] = u;
+    if (sp == 0 && R0 < rows) {
+      const int64_t block = (int64_t)unit * a.qi.blocks + R0 / 32;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) a.qi.img[(block * KS + kk) * 64 + lane] = q[r][kk];
+      if (lane == 0) a.qi.odd[block] = odd;
+      if (g == 0 && R < rows) a.qi.unit[(int64_t)unit * rows + R] = u;
+    }
   }
-  odd_q = __builtin_amdgcn_ballot_w64(odd_q) != 0;
   // keys every row of the wave attends (its first row's)
   const int R0 = blk * kStatRows + wave * 64;
   const int lim_wave = R0 < rows ? row_limit(a, R0, len) : 0x7fffffff;
@@ -146,7 +137,7 @@ void row_stats_kernel(const SumArgs a) {
       const int piece = KP * part + j;
       uint4 rest;
       uint4* dst = img[buf] + ((key >> 5) * KS + (piece >> 1)) * 64 + 32 * (piece & 1) + (key & 31);
-      *dst = decode<TWO>(raw[j], s, &rest);
+      *dst = decode<TWO, !TWO>(raw[j], s, &rest);
       if constexpr (TWO) dst[IMG] = rest;
     }
     if (part == 0) back[buf][key] = 1.0f / u;
@@ -265,16 +256,19 @@ __global__ __launch_bounds__(256) void row_merge_kernel(const SumArgs a, int64_t
 }
 
 // KB = 32-key blocks a wave keeps in registers (TWO: one, whose two terms take
-// the registers of two).
-template <int D, bool QF16, bool TWO>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+// the registers of two). The products of one 32 x 32 block of scores are issued
+// between the exponentials of the block before: matrix instructions hide the
+// vector work of their own wave only.
+template <int D, bool TWO>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void key_sums_kernel(const SumArgs a) {
   constexpr int KS = D / 16, KB = TWO ? 1 : 2;
-  constexpr int KEYS = 4 * 32 * KB;  // keys of a workgroup
-  constexpr int PC = 2 * KS / 4;     // pieces of a row tile that a thread brings in
-  __shared__ __align__(16) uint4 img[2][2 * KS * 64];
+  constexpr int KEYS = 4 * 32 * KB;      // keys of a workgroup
+  constexpr int IMG = 2 * KS * 64;       // 16-byte pieces of a row tile
+  constexpr int PC = IMG / 256;          // of them a thread's
+  constexpr int NM = KS * (TWO ? 2 : 1); // products of a block
+  __shared__ __align__(16) uint4 img[2][IMG];
   __shared__ __align__(16) float4 row_lds[2][kTile];  // (m, 1 / l, c / unit, limit as bits)
-  __shared__ int odd_lds[2][4];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -296,6 +290,34 @@ void key_sums_kernel(const SumArgs a) {
   }
   const int lo = max(ch * kSumRowTiles, first), hi = min((ch + 1) * kSumRowTiles, (rows + kTile - 1) / kTile);
 
+  // row tiles: thread tid brings pieces tid, tid + 256, ...
+  const float c = fmaxf(fabsf(a.b.scale_log2), 1.0e-30f);
+  const uint4* qi = a.qi.img + (int64_t)unit * a.qi.blocks * KS * 64 + tid;
+  const int* q_odd = a.qi.odd + (int64_t)unit * a.qi.blocks;
+  uint4 raw[PC];
+  float4 st_raw;
+  int odd_next = 0;  // of the tile in `raw`
+  auto load = [&](int t) {
+#pragma unroll
+    for (int x = 0; x < PC; ++x) {
+      const int rb = x / (PC / 2);  // (past the last block: the last, weighed 0)
+      raw[x] = qi[(int64_t)min(2 * t + rb, a.qi.blocks - 1) * KS * 64 + 256 * (x % (PC / 2))];
+    }
+    odd_next = q_odd[min(2 * t, a.qi.blocks - 1)] | q_odd[min(2 * t + 1, a.qi.blocks - 1)];
+    // (a row that weighs nothing, or is past the last: 2^(s - 3e38) times 0)
+    const int R = t * kTile + lane, Rc = min(R, rows - 1);
+    const float2 st = a.stats[(int64_t)unit * rows + Rc];
+    const bool on = R < rows && st.y > 0.0f;
+    st_raw = make_float4(on ? st.x : 3.0e38f, on ? st.y : 0.0f, c / a.qi.unit[(int64_t)unit * rows + Rc],
+                         __builtin_bit_cast(float, row_limit(a, R, len)));
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int x = 0; x < PC; ++x) img[buf][tid + 256 * x] = raw[x];
+    if (wave == 0) row_lds[buf][lane] = st_raw;
+  };
+  if (lo < hi) load(lo);
+
   // this wave's keys as the A operand
   const uint8_t* kp = a.b.kp + b * a.b.kps_b + kvh * a.b.kps_h;
   const uint16_t* ks = (const uint16_t*)a.b.ks + b * a.b.kss_b + kvh * a.b.kss_h;
@@ -313,7 +335,7 @@ void key_sums_kernel(const SumArgs a) {
       const uint32_t w = *(const uint32_t*)(kp + j * (D / 2) + 4 * (2 * kk + g));
       const _Float16 s = (_Float16)(scale_at(sraw, 16 * kk / a.b.G, a.s_f16) * u);
       uint4 rest;
-      k[kb][kk] = decode<TWO>(w, s, &rest);
+      k[kb][kk] = decode<TWO, !TWO>(w, s, &rest);
       if constexpr (TWO) k[kb][KS + kk] = rest;
     }
     const float ub = 1.0f / u;
@@ -322,106 +344,81 @@ void key_sums_kernel(const SumArgs a) {
   }
   odd_k = __builtin_amdgcn_ballot_w64(odd_k) != 0;
 
-  // row tiles: wave w brings the pieces of steps w, w + 4 of both 32-row blocks
-  const float c = fmaxf(fabsf(a.b.scale_log2), 1.0e-30f);
-  const uint32_t qneg = a.b.scale_log2 < 0.0f ? 0x80008000u : 0u;
-  uint4 raw[PC];
-  float unit_raw[2];
-  float4 st_raw;
-  auto load = [&](int t) {
-#pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
-      const int R = min(t * kTile + 32 * rb + n, rows - 1);
-      const int i = R / a.b.ratio, h = kvh * a.b.ratio + R % a.b.ratio;
-      const uint16_t* p = (const uint16_t*)a.b.q + b * a.b.qs_b + (int64_t)h * a.b.qs_h + (int64_t)i * a.b.qs_s + 8 * g;
-      // (a row that weighs nothing enters as zeros, whatever it holds)
-      unit_raw[rb] = a.stats[(int64_t)unit * rows + R].y > 0.0f ? a.row_unit[(int64_t)unit * rows + R] : 0.0f;
-#pragma unroll
-      for (int x = 0; x < PC / 2; ++x) raw[rb * (PC / 2) + x] = load_query(p + 16 * (wave + 4 * x), a.q_vec);
-    }
-    if (tid < kTile) {
-      const int R = t * kTile + tid, Rc = min(R, rows - 1);
-      const float2 st = a.stats[(int64_t)unit * rows + Rc];
-      const int lim = row_limit(a, R, len);  // (0 past the last row)
-      st_raw = make_float4(st.x, R < rows ? st.y : 0.0f, c / a.row_unit[(int64_t)unit * rows + Rc],
-                           __builtin_bit_cast(float, lim));
-    }
-  };
-  auto store = [&](int buf) {
-    bool odd = false;
-#pragma unroll
-    for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-      for (int x = 0; x < PC / 2; ++x) {
-        uint4 v = raw[rb * (PC / 2) + x];
-        const uint32_t top = QF16 ? 0x7c00u : 0x7f80u;
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int y = 0; y < 4; ++y) odd = odd || (w[y] & top) == top || ((w[y] >> 16) & top) == top;
-        const uint32_t keep = unit_raw[rb] > 0.0f ? 0xffffffffu : 0u;
-        v = make_uint4((v.x & keep) ^ qneg, (v.y & keep) ^ qneg, (v.z & keep) ^ qneg, (v.w & keep) ^ qneg);
-        img[buf][(rb * KS + wave + 4 * x) * 64 + lane] = query_piece<QF16>(v, unit_raw[rb]);
-      }
-    if (tid < kTile) row_lds[buf][tid] = st_raw;
-    const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
-    if (lane == 0) odd_lds[buf][wave] = any;
-  };
-
   float sum[KB][16];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int x = 0; x < 16; ++x) sum[kb][x] = 0.0f;
+  int odd = odd_k;
   if (lo < hi) {
-    load(lo);
     store(0);
+    odd = odd_k | odd_next;
     if (lo + 1 < hi) load(lo + 1);
   }
   __syncthreads();
+
+  // the block before: its scores, rows and whether it needs the rare path
+  f32x16_t s_old;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) s_old[x] = -__builtin_inff();
+  float4 r_old = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
+  bool rare_old = false;
+  // scores that are not finite, and keys that a row does not attend, of keys k_first ..
+  auto rare = [&](f32x16_t& s, const float (&bk)[16], float lim, int k_first) {
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      float u = bk[x];
+      asm volatile("" : "+v"(u));  // (nothing of the rare path is computed ahead, in registers of the loop)
+      const float inv = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, u));
+      s[x] = fminf(block_score(s[x] * u) * inv, 3.0e38f);
+      if (k_first + 8 * (x >> 2) + 4 * g + (x & 3) >= __builtin_bit_cast(int, lim)) s[x] = -__builtin_inff();
+    }
+  };
+  auto weigh = [&](const f32x16_t& s, const float (&bk)[16], const float4& r, float (&to)[16], int x) {
+    to[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x] * bk[x], r.z, -r.x)), r.y, to[x]);
+  };
+#pragma unroll 1
   for (int t = lo; t < hi; ++t) {
     const int cur = (t - lo) & 1;
+    const int odd_cur = odd;
     if (t + 1 < hi) {
       store(cur ^ 1);
+      odd = odd_k | odd_next;
       if (t + 2 < hi) load(t + 2);
     }
-    const bool odd = odd_k || (odd_lds[cur][0] | odd_lds[cur][1] | odd_lds[cur][2] | odd_lds[cur][3]) != 0;
     // the fewest keys a row of the tile attends: its first row's
     const int lim_tile = row_limit(a, t * kTile, len);
+    const uint4* qt = img[cur] + lane;
 #pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
-      const float4 rs = row_lds[cur][32 * rb + n];
-      const float m = rs.x, inv = rs.y, cr = rs.z;
-      const int lim = __builtin_bit_cast(int, rs.w);
+    for (int j = 0; j < 2 * KB; ++j) {
+      const int rb = j / KB, kb = j % KB, kb_old = (j + KB - 1) % KB;
+      if (rare_old) rare(s_old, back[kb_old], r_old.w, kw + 32 * kb_old);
+      f32x16_t s;
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        f32x16_t s;
+      for (int x = 0; x < 16; ++x) s[x] = 0.0f;
+      uint4 f[2];
+      f[0] = qt[rb * KS * 64];
 #pragma unroll
-        for (int x = 0; x < 16; ++x) s[x] = 0.0f;
+      for (int x = 0; x < NM; ++x) {
+        const int kk = TWO ? x / 2 : x;
+        if ((!TWO || x % 2 == 0) && kk + 1 < KS) f[(kk + 1) & 1] = qt[(rb * KS + kk + 1) * 64];
+        s = mfma(k[kb][TWO && x % 2 == 1 ? KS + kk : kk], f[kk & 1], s);
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-          const uint4 q = img[cur][(rb * KS + kk) * 64 + lane];
-          s = mfma(k[kb][kk], q, s);
-          if constexpr (TWO) s = mfma(k[kb][KS + kk], q, s);
+        for (int y = 0; y < 16 / NM; ++y) {
+          weigh(s_old, back[kb_old], r_old, sum[kb_old], x * (16 / NM) + y);
+          asm volatile("" : "+v"(sum[kb_old][x * (16 / NM) + y]));  // (here, not where the sums are next read)
         }
-#pragma unroll
-        for (int x = 0; x < 16; ++x) s[x] *= back[kb][x];
-        if (odd) {
-#pragma unroll
-          for (int x = 0; x < 16; ++x) s[x] = block_score(s[x]);
-        }
-        if (kw + 32 * (kb + 1) > lim_tile || (t + 1) * kTile > rows) {
-#pragma unroll
-          for (int x = 0; x < 16; ++x)
-            if (kw + 32 * kb + 8 * (x >> 2) + 4 * g + (x & 3) >= lim) s[x] = -__builtin_inff();
-        }
-#pragma unroll
-        for (int x = 0; x < 16; ++x)
-          sum[kb][x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], cr, -m)), inv, sum[kb][x]);
-        __builtin_amdgcn_sched_barrier(0);  // (one score block at a time: registers)
+        __builtin_amdgcn_sched_barrier(0);
       }
+      s_old = s;
+      r_old = row_lds[cur][32 * rb + n];
+      rare_old = odd_cur || kw + 32 * (kb + 1) > lim_tile;
     }
     __syncthreads();
   }
+  if (rare_old) rare(s_old, back[KB - 1], r_old.w, kw + 32 * (KB - 1));
+#pragma unroll
+  for (int x = 0; x < 16; ++x) weigh(s_old, back[KB - 1], r_old, sum[KB - 1], x);
   // over the 32 lanes of a key's rows
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
@@ -446,23 +443,13 @@ __global__ __launch_bounds__(256) void key_add_kernel(const SumArgs a) {
   a.weights[b * a.w_b + kvh * a.w_h + j * a.w_k] += v;
 }
 
-template <int D, bool QF16, bool TWO>
-void launch(const SumArgs& a, hipStream_t st) {
-  const int64_t rows = (int64_t)a.n_units * a.b.ratio * a.b.T;
-  hipLaunchKernelGGL((row_stats_kernel<D, QF16, TWO>), dim3((unsigned)((int64_t)a.n_units * a.row_blocks * a.splits)),
-                     dim3(256), 0, st, a);
-  hipLaunchKernelGGL(row_merge_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, a, rows);
-  hipLaunchKernelGGL((key_sums_kernel<D, QF16, TWO>), dim3((unsigned)((int64_t)a.n_units * a.key_blocks * a.chunks)),
-                     dim3(256), 0, st, a);
-  hipLaunchKernelGGL(key_add_kernel, dim3((unsigned)((a.b.Sk + 255) / 256), (unsigned)a.n_units), dim3(256), 0, st, a);
-}
-
 struct SumPlan {
-  int64_t row_blocks, splits, key_blocks, chunks;
-  int64_t part, unit, stats, sums;  // bytes
+  int64_t row_blocks, splits, key_blocks, chunks, q_blocks;
+  int64_t unit, img, odd, stats, scratch;  // bytes
+  RowsPlan rows;
 };
 
-SumPlan sum_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t Sk, bool two) {
+SumPlan sum_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool two, bool attend) {
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
   const int64_t rows = T * (Hq / Hkv), units = B * Hkv, keys = two ? 128 : 256;
   SumPlan p;
@@ -470,25 +457,52 @@ SumPlan sum_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t Sk, bool
   p.splits = std::max<int64_t>(1, ((Sk + kTile - 1) / kTile + kStatTiles - 1) / kStatTiles);
   p.key_blocks = (Sk + keys - 1) / keys;
   p.chunks = ((rows + kTile - 1) / kTile + kSumRowTiles - 1) / kSumRowTiles;
-  p.part = up(units * rows * p.splits * 8);
+  p.q_blocks = (rows + 31) / 32;
   p.unit = up(units * rows * 4);
+  p.img = units * p.q_blocks * 32 * D * 2;
+  p.odd = up(units * p.q_blocks * 4);
   p.stats = up(units * rows * 8);
-  p.sums = up(units * p.chunks * Sk * 4);
+  // one after the other: the first pass's partials, the second's sums
+  p.scratch = units * p.chunks * Sk * 4;
+  if (attend) {
+    p.rows = rows_plan(B, Hq, Hkv, T, D, Sk, true);
+    p.scratch = std::max(p.scratch, p.rows.ml_bytes + p.rows.o_bytes);
+  } else {
+    p.scratch = std::max(p.scratch, units * rows * p.splits * 8);
+  }
   return p;
+}
+
+template <int D, bool QF16, bool TWO>
+void launch_stats(const SumArgs& a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.n_units * a.b.ratio * a.b.T;
+  hipLaunchKernelGGL((row_stats_kernel<D, QF16, TWO>), dim3((unsigned)((int64_t)a.n_units * a.row_blocks * a.splits)),
+                     dim3(256), 0, st, a);
+  hipLaunchKernelGGL(row_merge_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, a, rows);
+}
+
+template <int D, bool TWO>
+void launch_sums(const SumArgs& a, bool stats, hipStream_t st) {
+  if (stats) {
+    if (a.b.q_dt == KVQ_F16) launch_stats<D, true, TWO>(a, st);
+    else launch_stats<D, false, TWO>(a, st);
+  }
+  hipLaunchKernelGGL((key_sums_kernel<D, TWO>), dim3((unsigned)((int64_t)a.n_units * a.key_blocks * a.chunks)),
+                     dim3(256), 0, st, a);
+  hipLaunchKernelGGL(key_add_kernel, dim3((unsigned)((a.b.Sk + 255) / 256), (unsigned)a.n_units), dim3(256), 0, st, a);
 }
 
 }  // namespace
 
-int64_t sums_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t Sk, bool s_f16) {
-  const SumPlan p = sum_plan(B, Hq, Hkv, T, Sk, s_f16);
-  return p.part + p.unit + p.stats + p.sums;
+int64_t sums_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool s_f16, bool attend) {
+  const SumPlan p = sum_plan(B, Hq, Hkv, T, D, Sk, s_f16, attend);
+  return p.unit + p.img + p.odd + p.stats + p.scratch;
 }
 
-int launch_key_sums(const BlockArgs& b, float* weights, const int64_t* ws, void* workspace, hipStream_t st) {
+int launch_key_sums(const BlockArgs& b, bool attend, float* weights, const int64_t* ws, void* workspace, hipStream_t st) {
   const bool two = b.s_dt == KVQ_F16;
-  const SumPlan p = sum_plan(b.B, b.Hq, b.Hkv, b.T, b.Sk, two);
+  const SumPlan p = sum_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk, two, attend);
   const int64_t units = (int64_t)b.B * b.Hkv;
-  if (b.Sk == 0) return KVQ_OK;
   if (units * p.row_blocks * p.splits >= (int64_t(1) << 31) || units * p.key_blocks * p.chunks >= (int64_t(1) << 31) ||
       units >= 65536 || (int64_t)b.T * b.ratio >= (int64_t(1) << 30))
     return KVQ_EUNSUP;
@@ -501,20 +515,32 @@ int launch_key_sums(const BlockArgs& b, float* weights, const int64_t* ws, void*
   a.row_blocks = (int)p.row_blocks; a.splits = (int)p.splits;
   a.key_blocks = (int)p.key_blocks; a.chunks = (int)p.chunks;
   char* w = (char*)workspace;
+  a.qi.img = (uint4*)w;
+  w += p.img;
+  a.qi.unit = (float*)w;
+  w += p.unit;
+  a.qi.odd = (int*)w;
+  a.qi.blocks = (int)p.q_blocks;
+  w += p.odd;
+  a.stats = (float2*)w;
+  w += p.stats;
   a.part = (float2*)w;
-  a.row_unit = (float*)(w + p.part);
-  a.stats = (float2*)(w + p.part + p.unit);
-  a.sums = (float*)(w + p.part + p.unit + p.stats);
+  a.sums = (float*)w;
   a.weights = weights;
   a.w_b = ws[0]; a.w_h = ws[1]; a.w_k = ws[2];
-  const bool f16 = b.q_dt == KVQ_F16;
-  if (b.D == 128) {
-    if (f16) two ? launch<128, true, true>(a, st) : launch<128, true, false>(a, st);
-    else two ? launch<128, false, true>(a, st) : launch<128, false, false>(a, st);
-  } else {
-    if (f16) two ? launch<64, true, true>(a, st) : launch<64, true, false>(a, st);
-    else two ? launch<64, false, true>(a, st) : launch<64, false, false>(a, st);
+  if (attend) {
+    RowsArgs r = {};
+    fill_block_mfma(&r.m, b);
+    r.m.b.stats = a.stats;
+    r.m.ws_ml = (float2*)w;
+    r.m.ws_o = (float*)(w + p.rows.ml_bytes);
+    r.qi = a.qi;
+    const int rc = launch_rows(r, p.rows, st);
+    if (rc != KVQ_OK) return rc;
   }
+  if (b.Sk == 0) return KVQ_OK;
+  if (b.D == 128) two ? launch_sums<128, true>(a, !attend, st) : launch_sums<128, false>(a, !attend, st);
+  else two ? launch_sums<64, true>(a, !attend, st) : launch_sums<64, false>(a, !attend, st);
   return KVQ_OK;
 }
 

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(kRowThreads) void block_rows_kernel(const BlockArgs
 #pragma unroll
   for (int w = 0; w < kRowThreads / 64; ++w) l += red[w];
   if (a.stats && tid == 0)
-    a.stats[((int64_t)b * a.Hq + h) * a.T + i] = make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
+    a.stats[stats_at(a, b, h, i)] = make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
   if (a.out && tid < a.D) {
     float x = 0.0f;
     for (int w = 0; w < parts; ++w) x += o_lds[w * a.D + tid];
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(kRowThreads) void block_rows8_kernel(const BlockArg
 #pragma unroll
   for (int w = 0; w < kRowThreads / 64; ++w) l += red[w];
   if (a.stats && tid == 0)
-    a.stats[((int64_t)b * a.Hq + h) * a.T + i] = make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
+    a.stats[stats_at(a, b, h, i)] = make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
   if (a.out && tid < a.D) {
     float x = 0.0f;
     for (int y = 0; y < parts; ++y) x += o_lds[(y * words) * 8 + tid];

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(kWThreads) void key_weights_rows_kernel(const Block
   float sum = 0.0f;
   for (int R = part; R < a.ratio * a.T; R += kWThreads / kWKeys) {
     const int i = R / a.ratio, h = kvh * a.ratio + R % a.ratio;
-    const float2 st = a.stats[((int64_t)b * a.Hq + h) * a.T + i];
+    const float2 st = a.stats[stats_at(a, b, h, i)];
     if (st.y == 0.0f || j >= len || (j >= base && !block_sees(a, b, i, j - base))) continue;
     const int64_t q0 = b * a.qs_b + h * a.qs_h + i * a.qs_s;
     float s = 0.0f;
@@ -88,8 +88,7 @@ int64_t workspace_needed(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t 
   int64_t n = stats_bytes(B, Hq, T);
   if (B == 0 || T == 0 || !(D == 64 || D == 128) || q_dt == KVQ_F32 || s_dt == KVQ_F32) return n;
   if (with_out && takes_scores(B, Hq, Hkv, T, D, Sk, q_dt, s_dt)) return std::max(n, block_scores_bytes(B, Hq, Hkv, T, D, Sk));
-  n = std::max(n, sums_workspace_bytes(B, Hq, Hkv, T, Sk, s_dt == KVQ_F16));
-  if (with_out) n = std::max(n, block_workspace_bytes(B, Hq, Hkv, T, D, Sk));
+  n = std::max(n, sums_workspace_bytes(B, Hq, Hkv, T, D, Sk, s_dt == KVQ_F16, with_out));
   return n;
 }
 
@@ -130,17 +129,10 @@ int weights_impl(const char* what, const void* q, int q_dtype, const int64_t* q_
     return KVQ_OK;
   }
   if (block_mfma_takes_keys(a)) {
-    // attention, then the sums, in the same workspace one after the other
     a.stats = nullptr;
-    if (a.out) {
-      if (block_mfma_takes(a)) {
-        const int lc = launch_block_mfma(a, workspace, workspace_bytes, st);
-        KVQ_CHECK_ARG(lc == KVQ_OK, "%s: too large", what);
-      } else {
-        launch_block_rows(a, st);
-      }
-    }
-    const int lc = launch_key_sums(a, weights, weight_strides, workspace, st);
+    const bool attend = a.out && block_mfma_takes(a);
+    if (a.out && !attend) launch_block_rows(a, st);
+    const int lc = launch_key_sums(a, attend, weights, weight_strides, workspace, st);
     KVQ_CHECK_ARG(lc == KVQ_OK, "%s: too large", what);
   } else {
     launch_block_rows(a, st);

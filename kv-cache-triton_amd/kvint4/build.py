@@ -31,7 +31,8 @@ SOURCES = ("kvq_capi.hip", "kvq_quant.hip", "kvq_attn.hip", "kvq_prefill.hip", "
 SOURCE_FLAGS = {"kvq_attn.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true"),
                 "kvq_prefill.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true"),
                 "kvq_block.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true"),
-                "kvq_rows.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true")}
+                "kvq_rows.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true"),
+                "kvq_sums.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=true")}
 # gfx950 only: the decode kernels assume its wave64 MFMA forms and its
 # round-robin workgroup-to-XCD dispatch (checked again at run time).
 ARCH = "gfx950"

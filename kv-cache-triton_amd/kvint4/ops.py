@@ -1263,8 +1263,10 @@ def attention_with_key_weights(
     _check_cache(what, q, (k_packed, k_scales, v_packed, v_scales), B, n_kv_heads, D, group_size)
     Sk = k_packed.shape[2]
     _check_weights(what, key_weights, B, n_kv_heads, Sk)
-    if seq_lens is None and use_prefill_kernel(Hq // n_kv_heads * Sq, Sk):
-        # long blocks: the prefill kernels, and the weights beside them
+    # long blocks that the kernel with both does not take on the matrix cores:
+    # the prefill kernels, and the weights beside them
+    matrix = D in (64, 128) and group_size in (32, 64, 128) and torch.float32 not in (q.dtype, k_scales.dtype)
+    if not matrix and seq_lens is None and use_prefill_kernel(Hq // n_kv_heads * Sq, Sk):
         try:
             prefill_attention(q, k_packed, k_scales, v_packed, v_scales, n_kv_heads=n_kv_heads, group_size=group_size,
                               is_causal=is_causal, sm_scale=sm_scale, out=out)
