@@ -805,9 +805,9 @@ int launch_any(const BlockMfmaArgs& a, const BlockPlan& p, hipStream_t st) {
 
 }  // namespace
 
-int64_t block_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk) {
-  if (T * (Hq / Hkv) > kRowsMin) {
-    const RowsPlan p = rows_plan(B, Hq, Hkv, T, D, Sk, false);
+int64_t block_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool s_f16) {
+  if (T * (Hq / Hkv) > rows_min(s_f16)) {
+    const RowsPlan p = rows_plan(B, Hq, Hkv, T, D, Sk, s_f16, false);
     return p.ml_bytes + p.o_bytes;
   }
   const BlockPlan p = block_plan(B, Hq, Hkv, T, D, Sk);
@@ -816,9 +816,9 @@ int64_t block_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int
 
 int launch_block_mfma(const BlockArgs& b, void* workspace, int64_t workspace_bytes, hipStream_t st) {
   const bool fits = workspace != nullptr && (uintptr_t)workspace % 16 == 0 &&
-                    workspace_bytes >= block_workspace_bytes(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk);
-  if ((int64_t)b.T * b.ratio > kRowsMin) {
-    RowsPlan p = rows_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk, false);
+                    workspace_bytes >= block_workspace_bytes(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk, b.s_dt == KVQ_F16);
+  if ((int64_t)b.T * b.ratio > rows_min(b.s_dt == KVQ_F16)) {
+    RowsPlan p = rows_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk, b.s_dt == KVQ_F16, false);
     if (!fits) p.n_split = 1;
     RowsArgs a = {};
     fill_block_mfma(&a.m, b);

@@ -36,7 +36,7 @@ bool block_mfma_takes(const BlockArgs& a);
 
 // Attention by the kernel of few rows or of many; without the workspace for its
 // split the launch does not split.
-int64_t block_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk);
+int64_t block_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool s_f16);
 int launch_block_mfma(const BlockArgs& b, void* workspace, int64_t workspace_bytes, hipStream_t st);
 
 // Attention that keeps its scores, and the key weights from them, for up to
@@ -58,7 +58,7 @@ struct QueryImages {
 
 // Many rows per KV head (kvq_rows.hip): the arguments of the kernel, its plan
 // and launch. With qi.img it keeps the query operands and sums the softmax in
-// full precision; `two`: such a launch on fp16 scales.
+// full precision.
 struct RowsArgs {
   BlockMfmaArgs m;
   QueryImages qi;
@@ -69,8 +69,14 @@ struct RowsPlan {
   int64_t row_chunks, n_split, ml_bytes, o_bytes;
 };
 
-constexpr int64_t kRowsMin = 32;  // more rows per KV head than this take it
-RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool weights);
+// Trees of more rows per KV head than this take it. Where the keys fill the GPU
+// it is faster from 65 rows (104 rows of 64 KV heads over 8K keys: 57 against 82
+// us by kvq_block.hip), and never by more than 4 us slower (96 rows of 8 heads
+// over 16K keys: 34.5 against 33.4; 256 rows: 45 against 54). With fp16 scales,
+// two products each: 128 rows of 16 heads over 30K keys 94 against 80 us, 404
+// rows 183 against 257.
+inline int64_t rows_min(bool s_f16) { return s_f16 ? 128 : 64; }
+RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool s_f16, bool weights);
 int launch_rows(RowsArgs a, const RowsPlan& p, hipStream_t st);
 
 // Key weights of blocks of any length (kvq_sums.hip), for what

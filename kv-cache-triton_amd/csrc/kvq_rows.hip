@@ -1,6 +1,6 @@
 // Attention of many query rows over the INT4 cache on the matrix cores
-// (gfx950): trees and blocks of more than kRowsMin rows per KV head, and the
-// prompts whose key weights are counted, for 16-bit queries and scales, D 64
+// (gfx950): trees of more than rows_min rows per KV head, and the blocks whose key
+// weights are counted but for those of few rows, for 16-bit queries and scales, D 64
 // and 128, aligned rows.
 //
 // A wave takes 32 query rows, a workgroup of NW waves 32 NW rows of one KV head
@@ -8,10 +8,11 @@
 // LDS images in the order the matrix operands are read, and every wave reads
 // them from there (conflict-free 16-byte reads). v_mfma 32x32x16, fp16 operands:
 //   S^T = K Q^T, O^T += V^T P^T.
-// Scores are exact to fp32's rounding for bf16 scales, and for fp16 scales with
-// TWO (kvq_operands.h). Scales enter times one power of two for the keys and one
-// for the values; the rare key whose scale fp16 does not hold even so has its
-// score, or its share of the output, formed in fp32.
+// Scores are exact to fp32's rounding: fp16 scales take two products
+// (kvq_operands.h). Scales enter times one power of two for the keys and one for
+// the values; the rare key whose scale fp16 does not hold even so has its score,
+// or its share of the output, formed in fp32. Values times fp16 scales, and the
+// weights, are rounded to fp16 (2^-12, near the output's own rounding or under it).
 //
 // In iteration i a wave's matrix instructions and vector work come in two pairs
 // that do not wait for each other: S(i) with the decoding of tile i + 1's keys
@@ -39,12 +40,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* p, uint32_
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
 }
 
-// SUMS: for key weights: the sums of the softmax in fp32 (as the products take
-// them, else), the query operands kept, and both terms of fp16 scales (TWO).
+// SUMS: for key weights, the query operands are kept, and the softmax sums the
+// weights as they are. Else, with bf16 scales (whose values are exact in fp16), it
+// sums the rounded weights that the products take, two in an instruction.
 template <int D, bool QF16, bool SF16, bool SUMS, int NW, bool PAGED>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void rows_attn_kernel(const RowsArgs a) {
-  constexpr bool TWO = SUMS && SF16;
+  constexpr bool TWO = SF16;
   constexpr int NT = 64 * NW, ROWS = 32 * NW;
   constexpr int KS = D / 16;           // 16-dim steps of S^T
   constexpr int NDB = D / 32;          // 32-dim blocks of O^T
@@ -412,7 +414,7 @@ void rows_attn_kernel(const RowsArgs a) {
           const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], cr, -m_run));
           const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r + 1], cr, -m_run));
           const f16x2_t h = {(_Float16)e0, (_Float16)e1}, one = {(_Float16)1.0f, (_Float16)1.0f};
-          if constexpr (SUMS) ls += e0 + e1;
+          if constexpr (SUMS || SF16) ls += e0 + e1;
           else ls = __builtin_amdgcn_fdot2(h, one, ls, false);
           ((uint32_t*)&pc[w >> 2])[w & 3] = u32_of(h);
         }
@@ -532,8 +534,8 @@ void launch(const RowsArgs& a, hipStream_t st) {
 template <int D, bool QF16, bool SF16>
 void launch_waves(const RowsArgs& a, int nw, hipStream_t st) {
   if (a.qi.img) launch<D, QF16, SF16, true, 8>(a, st);
-  else if (nw == 8) launch<D, QF16, SF16, false, 8>(a, st);
-  else launch<D, QF16, SF16, false, 4>(a, st);
+  else if (SF16 || nw == 8) launch<D, QF16, SF16, false, 8>(a, st);
+  else if constexpr (!SF16) launch<D, QF16, SF16, false, 4>(a, st);
 }
 
 template <int D>
@@ -545,13 +547,13 @@ void launch_types(const RowsArgs& a, int nw, hipStream_t st) {
 
 }  // namespace
 
-RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool weights) {
+RowsPlan rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool s_f16, bool weights) {
   const int64_t rows = T * (Hq / Hkv), units = B * Hkv, tiles = (Sk + kTile - 1) / kTile;
   RowsPlan p;
   // eight waves (256 rows, one workgroup per CU), or four, two workgroups per
-  // CU, where eight would leave four without rows; key weights are
-  // of prompts, with rows enough
-  p.nw = weights || (rows + 127) / 128 % 2 == 0 || rows > 1024 ? 8 : 4;
+  // CU, where eight would leave four without rows. Key weights are of prompts,
+  // with rows enough, and two terms take the LDS of eight waves' workgroup.
+  p.nw = weights || s_f16 || (rows + 127) / 128 % 2 == 0 || rows > 1024 ? 8 : 4;
   p.row_chunks = (rows + 32 * p.nw - 1) / (32 * p.nw);
   // the split with the least estimate, in tiles' times (2.2 us): rounds of the
   // workgroups that are resident together, each its tiles and about six tiles'

@@ -33,14 +33,13 @@ constexpr float kNeg = -1.0e30f;
 constexpr float kLazyMax = 8.0f;
 constexpr int kStatRows = 256;   // rows of a workgroup of the first pass (64 a wave)
 constexpr int kStatTiles = 16;   // key tiles of its share
-constexpr int kSumRowTiles = 16; // row tiles of a share of the second pass
 
 struct SumArgs {
   BlockArgs b;
   QueryImages qi;
   int n_units, ng, s_f16, q_vec;
   int row_blocks, splits;  // first pass: row blocks, shares of the keys
-  int key_blocks, chunks;  // second pass: key blocks, shares of the rows
+  int key_blocks, chunks, chunk_tiles;  // second pass: key blocks, shares of the rows, row tiles of a share
   float2* part;            // [unit][row][split] (m, l)
   float2* stats;           // [unit][row] (m, 1 / l)
   float* sums;             // [unit][chunk][Sk]
@@ -288,7 +287,11 @@ void key_sums_kernel(const SumArgs a) {
     const int64_t i = (int64_t)k0 - (len - a.b.T);
     first = i <= 0 ? 0 : (int)(i * a.b.ratio / kTile);
   }
-  const int lo = max(ch * kSumRowTiles, first), hi = min((ch + 1) * kSumRowTiles, (rows + kTile - 1) / kTile);
+  const int lo = max(ch * a.chunk_tiles, first), hi = min((ch + 1) * a.chunk_tiles, (rows + kTile - 1) / kTile);
+  if (lo >= hi) {
+    for (int j = k0 + tid; j < min(k0 + KEYS, len); j += 256) dst[j] = 0.0f;
+    return;
+  }
 
   // row tiles: thread tid brings pieces tid, tid + 256, ...
   const float c = fmaxf(fabsf(a.b.scale_log2), 1.0e-30f);
@@ -316,7 +319,7 @@ void key_sums_kernel(const SumArgs a) {
     for (int x = 0; x < PC; ++x) img[buf][tid + 256 * x] = raw[x];
     if (wave == 0) row_lds[buf][lane] = st_raw;
   };
-  if (lo < hi) load(lo);
+  load(lo);
 
   // this wave's keys as the A operand
   const uint8_t* kp = a.b.kp + b * a.b.kps_b + kvh * a.b.kps_h;
@@ -349,12 +352,9 @@ void key_sums_kernel(const SumArgs a) {
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int x = 0; x < 16; ++x) sum[kb][x] = 0.0f;
-  int odd = odd_k;
-  if (lo < hi) {
-    store(0);
-    odd = odd_k | odd_next;
-    if (lo + 1 < hi) load(lo + 1);
-  }
+  store(0);
+  int odd = odd_k | odd_next;
+  if (lo + 1 < hi) load(lo + 1);
   __syncthreads();
 
   // the block before: its scores, rows and whether it needs the rare path
@@ -444,19 +444,39 @@ __global__ __launch_bounds__(256) void key_add_kernel(const SumArgs a) {
 }
 
 struct SumPlan {
-  int64_t row_blocks, splits, key_blocks, chunks, q_blocks;
+  int64_t row_blocks, splits, key_blocks, chunks, chunk_tiles, q_blocks;
   int64_t unit, img, odd, stats, scratch;  // bytes
   RowsPlan rows;
 };
 
-SumPlan sum_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool two, bool attend) {
+SumPlan sum_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool causal, bool two, bool attend) {
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
   const int64_t rows = T * (Hq / Hkv), units = B * Hkv, keys = two ? 128 : 256;
   SumPlan p;
   p.row_blocks = (rows + kStatRows - 1) / kStatRows;
   p.splits = std::max<int64_t>(1, ((Sk + kTile - 1) / kTile + kStatTiles - 1) / kStatTiles);
   p.key_blocks = (Sk + keys - 1) / keys;
-  p.chunks = ((rows + kTile - 1) / kTile + kSumRowTiles - 1) / kSumRowTiles;
+  // shares of the rows: the number of them with the least estimate, in tiles'
+  // times: rounds of the 512 workgroups that are resident together, each its
+  // tiles and about three tiles' time of prologue
+  const int64_t tiles = (rows + kTile - 1) / kTile, ratio = Hq / Hkv;
+  double best = 0.0;
+  p.chunks = p.chunk_tiles = 0;
+  for (const int64_t n : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
+    if (n > tiles) break;
+    const int64_t each = (tiles + n - 1) / n, shares = (tiles + each - 1) / each;
+    int64_t wgs = 0;  // that some row attends
+    for (int64_t x = 0; x < shares; ++x) {
+      const int64_t last = std::min((x + 1) * each * kTile, rows) - 1, seen = Sk - T + last / ratio + 1;
+      wgs += causal ? std::min(p.key_blocks, std::max<int64_t>(0, seen + keys - 1) / keys) : p.key_blocks;
+    }
+    const double cost = (double)((units * wgs + 511) / 512) * (double)(each + 3);
+    if (n == 1 || cost < best) {
+      best = cost;
+      p.chunks = shares;
+      p.chunk_tiles = each;
+    }
+  }
   p.q_blocks = (rows + 31) / 32;
   p.unit = up(units * rows * 4);
   p.img = units * p.q_blocks * 32 * D * 2;
@@ -465,7 +485,7 @@ SumPlan sum_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64
   // one after the other: the first pass's partials, the second's sums
   p.scratch = units * p.chunks * Sk * 4;
   if (attend) {
-    p.rows = rows_plan(B, Hq, Hkv, T, D, Sk, true);
+    p.rows = rows_plan(B, Hq, Hkv, T, D, Sk, two, true);
     p.scratch = std::max(p.scratch, p.rows.ml_bytes + p.rows.o_bytes);
   } else {
     p.scratch = std::max(p.scratch, units * rows * p.splits * 8);
@@ -495,13 +515,14 @@ void launch_sums(const SumArgs& a, bool stats, hipStream_t st) {
 }  // namespace
 
 int64_t sums_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t Sk, bool s_f16, bool attend) {
-  const SumPlan p = sum_plan(B, Hq, Hkv, T, D, Sk, s_f16, attend);
-  return p.unit + p.img + p.odd + p.stats + p.scratch;
+  // (the mask is the call's: as much as either needs)
+  const SumPlan c = sum_plan(B, Hq, Hkv, T, D, Sk, true, s_f16, attend), f = sum_plan(B, Hq, Hkv, T, D, Sk, false, s_f16, attend);
+  return c.unit + c.img + c.odd + c.stats + std::max(c.scratch, f.scratch);
 }
 
 int launch_key_sums(const BlockArgs& b, bool attend, float* weights, const int64_t* ws, void* workspace, hipStream_t st) {
   const bool two = b.s_dt == KVQ_F16;
-  const SumPlan p = sum_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk, two, attend);
+  const SumPlan p = sum_plan(b.B, b.Hq, b.Hkv, b.T, b.D, b.Sk, b.kind == kMaskCausal, two, attend);
   const int64_t units = (int64_t)b.B * b.Hkv;
   if (units * p.row_blocks * p.splits >= (int64_t(1) << 31) || units * p.key_blocks * p.chunks >= (int64_t(1) << 31) ||
       units >= 65536 || (int64_t)b.T * b.ratio >= (int64_t(1) << 30))
@@ -513,7 +534,7 @@ int launch_key_sums(const BlockArgs& b, bool attend, float* weights, const int64
   a.s_f16 = two;
   a.q_vec = (uintptr_t)b.q % 16 == 0 && b.qs_b % 8 == 0 && b.qs_h % 8 == 0 && b.qs_s % 8 == 0;
   a.row_blocks = (int)p.row_blocks; a.splits = (int)p.splits;
-  a.key_blocks = (int)p.key_blocks; a.chunks = (int)p.chunks;
+  a.key_blocks = (int)p.key_blocks; a.chunks = (int)p.chunks; a.chunk_tiles = (int)p.chunk_tiles;
   char* w = (char*)workspace;
   a.qi.img = (uint4*)w;
   w += p.img;

@@ -383,5 +383,5 @@ extern "C" int64_t kvq_tree_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t 
     return KVQ_EINVAL;
   }
   if (B == 0 || T == 0 || !(D == 64 || D == 128) || q_dtype == KVQ_F32 || scale_dtype == KVQ_F32) return 0;
-  return block_workspace_bytes(B, Hq, Hkv, T, D, Sk);
+  return block_workspace_bytes(B, Hq, Hkv, T, D, Sk, scale_dtype == KVQ_F16);
 }
