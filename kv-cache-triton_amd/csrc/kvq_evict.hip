@@ -238,11 +238,9 @@ struct MoveArgs {
 
 __device__ __forceinline__ int64_t move_first(const MoveArgs& a, int b) { return a.first ? a.first[b] : a.first0; }
 
-// Source and destination row of item i, or source -1 (nothing moves): an index
+// Source and destination row of an item, or source -1 (nothing moves): an index
 // outside [0, S), a destination outside its rows, a page without a block.
-__device__ __forceinline__ void move_rows_of(const MoveArgs& a, int b, int h, int i, int64_t* src, int64_t* dst) {
-  const int64_t from = a.index[b * a.is_b + h * a.is_h + i * a.is_i];
-  const int64_t to = move_first(a, b) + i;
+__device__ __forceinline__ void move_rows_of(const MoveArgs& a, int b, int64_t from, int64_t to, int64_t* src, int64_t* dst) {
   *src = -1;
   *dst = to;
   if (from < 0 || from >= a.S || to < 0 || to >= a.dst_rows) return;
@@ -276,6 +274,46 @@ __device__ __forceinline__ void move_store(uint8_t* p, int unit, uint4 v) {
 constexpr int kMoveThreads = 256;
 constexpr int kMovePer = 4;  // pieces a thread moves, all loads before the stores
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// Pieces of V's size: every load is issued before the first store, and none
+// under a condition (a piece that does not move reads row 0), so that all are in
+// flight together.
+template <typename V>
+__device__ __forceinline__ void move_pieces(const MoveArgs& a, const MoveTensor& t, int b, int h, uint32_t x0) {
+  const uint32_t pieces = (uint32_t)a.n * (uint32_t)t.lpr;
+  const int32_t* index = a.index + b * a.is_b + h * a.is_h;
+  const int64_t first = move_first(a, b);
+  int64_t s[kMovePer], d[kMovePer];
+  int at[kMovePer];
+  bool on[kMovePer];
+#pragma unroll
+  for (int y = 0; y < kMovePer; ++y) {
+    const uint32_t x = x0 + y * kMoveThreads, xc = x < pieces ? x : pieces - 1, i = fdiv(xc, t.div);
+    at[y] = (int)(xc - i * (uint32_t)t.lpr) * (int)sizeof(V);
+    s[y] = index[i * a.is_i];
+    d[y] = first + i;
+    on[y] = x < pieces;
+  }
+#pragma unroll
+  for (int y = 0; y < kMovePer; ++y) {
+    int64_t from, to;
+    move_rows_of(a, b, s[y], d[y], &from, &to);
+    on[y] = on[y] & (from >= 0);
+    s[y] = from < 0 ? 0 : from;
+    d[y] = to;
+  }
+  const uint8_t* src = t.src + b * t.ss_b + h * t.ss_h;
+  uint8_t* dst = t.dst + b * t.ds_b + h * t.ds_h;
+  V v[kMovePer];
+#pragma unroll
+  for (int y = 0; y < kMovePer; ++y) v[y] = *(const V*)(src + s[y] * t.ss_s + at[y]);
+#pragma unroll
+  for (int y = 0; y < kMovePer; ++y)
+    if (on[y]) *(V*)(dst + d[y] * t.ds_s + at[y]) = v[y];
+}
+
 // Into other buffers: a thread moves pieces of rows; a workgroup's tensor is
 // found from the workgroups of those before it, blockIdx.y is the (sequence,
 // head). Memory-bound, in pieces of up to 16 bytes of rows that lie apart.
@@ -286,25 +324,11 @@ __global__ __launch_bounds__(kMoveThreads) void move_rows_kernel(const MoveArgs 
   const MoveTensor& t = a.t[k];
   const int h = blockIdx.y % a.H, b = blockIdx.y / a.H;
   const uint32_t x0 = (blockIdx.x - a.wg0[k]) * (kMoveThreads * kMovePer) + threadIdx.x;
-  const uint32_t pieces = (uint32_t)a.n * (uint32_t)t.lpr;
-  int64_t s[kMovePer], d[kMovePer];
-  int at[kMovePer];
-#pragma unroll
-  for (int y = 0; y < kMovePer; ++y) {
-    const uint32_t x = x0 + y * kMoveThreads, i = fdiv(x, t.div);
-    at[y] = (int)(x - i * (uint32_t)t.lpr) * t.unit;
-    s[y] = -1;
-    if (x < pieces) move_rows_of(a, b, h, (int)i, &s[y], &d[y]);
-  }
-  const uint8_t* src = t.src + b * t.ss_b + h * t.ss_h;
-  uint8_t* dst = t.dst + b * t.ds_b + h * t.ds_h;
-  uint4 v[kMovePer];
-#pragma unroll
-  for (int y = 0; y < kMovePer; ++y)
-    if (s[y] >= 0) v[y] = move_load(src + s[y] * t.ss_s + at[y], t.unit);
-#pragma unroll
-  for (int y = 0; y < kMovePer; ++y)
-    if (s[y] >= 0) move_store(dst + d[y] * t.ds_s + at[y], t.unit, v[y]);
+  if (t.unit == 16) move_pieces<u32x4_t>(a, t, b, h, x0);
+  else if (t.unit == 8) move_pieces<u32x2_t>(a, t, b, h, x0);
+  else if (t.unit == 4) move_pieces<uint32_t>(a, t, b, h, x0);
+  else if (t.unit == 2) move_pieces<uint16_t>(a, t, b, h, x0);
+  else move_pieces<uint8_t>(a, t, b, h, x0);
 }
 
 // In place: one workgroup per tensor, sequence and head reads every row that
@@ -316,9 +340,11 @@ __global__ __launch_bounds__(kMoveThreads) void move_rows_in_place_kernel(const 
   const MoveTensor t = a.t[blockIdx.y];
   const int h = blockIdx.z % a.H, b = blockIdx.z / a.H;
   const int pieces = a.n * t.lpr;
+  const int32_t* index = a.index + b * a.is_b + h * a.is_h;
+  const int64_t first = move_first(a, b);
   for (int x = threadIdx.x; x < pieces; x += kMoveThreads) {
     int64_t s, d;
-    move_rows_of(a, b, h, x / t.lpr, &s, &d);
+    move_rows_of(a, b, index[(x / t.lpr) * a.is_i], first + x / t.lpr, &s, &d);
     if (s < 0) continue;
     move_store(lds + (int64_t)x * t.unit, t.unit,
                move_load(t.src + b * t.ss_b + h * t.ss_h + s * t.ss_s + (x % t.lpr) * t.unit, t.unit));
@@ -326,7 +352,7 @@ __global__ __launch_bounds__(kMoveThreads) void move_rows_in_place_kernel(const 
   __syncthreads();
   for (int x = threadIdx.x; x < pieces; x += kMoveThreads) {
     int64_t s, d;
-    move_rows_of(a, b, h, x / t.lpr, &s, &d);
+    move_rows_of(a, b, index[(x / t.lpr) * a.is_i], first + x / t.lpr, &s, &d);
     if (s < 0) continue;
     move_store(t.dst + b * t.ds_b + h * t.ds_h + d * t.ds_s + (x % t.lpr) * t.unit, t.unit,
                move_load(lds + (int64_t)x * t.unit, t.unit));
@@ -388,6 +414,7 @@ int move_impl(const char* what, int64_t n_tensors, const void* const* src, const
   }
   if (B == 0 || n == 0) return KVQ_OK;
   KVQ_CHECK_ARG(index, "%s: null index", what);
+  if (S == 0 || (pm && pm->n_blocks == 0)) return KVQ_OK;  // no row to move
   a.index = index;
   a.is_b = index_strides[0]; a.is_h = index_strides[1]; a.is_i = index_strides[2];
   a.first = first;

@@ -182,15 +182,16 @@ __global__ __launch_bounds__(kRowThreads) void block_rows_kernel(const BlockArgs
 
 // The same where groups are whole code words (G a multiple of 8, D too, and
 // rows aligned for 4-byte loads): a thread scores a key eight dims at a time,
-// and weighs eight dims of every (256 / (D / 8))-th key, so that no index is
+// and weighs eight dims of every (NT / (D / 8))-th key, so that no index is
 // divided in a loop and a chunk's loads are in flight together. (96 rows of
-// GPT-2 small over 1000 keys: 105 us above, 16 here.)
-__global__ __launch_bounds__(kRowThreads) void block_rows8_kernel(const BlockArgs a) {
+// GPT-2 small over 1000 keys: 105 us above, 23 with 256 threads, 13 with 1024.)
+template <int NT>
+__global__ __launch_bounds__(NT) void block_rows8_kernel(const BlockArgs a) {
   __shared__ __align__(16) float q_lds[kMaxBlockD];
-  __shared__ float p_lds[kRowThreads];
-  __shared__ int64_t row_lds[kRowThreads];
-  __shared__ float red[kRowThreads / 64];
-  __shared__ __align__(16) float o_lds[kRowThreads * 8];
+  __shared__ float p_lds[NT];
+  __shared__ int64_t row_lds[NT];
+  __shared__ float red[NT / 64];
+  __shared__ __align__(16) float o_lds[NT * 8];
   const int tid = threadIdx.x, wave = tid >> 6;
   int wg = blockIdx.x;
   const int i = wg % a.T;
@@ -206,10 +207,10 @@ __global__ __launch_bounds__(kRowThreads) void block_rows8_kernel(const BlockArg
   const uint8_t* kp = a.kp + b * a.kps_b + kvh * a.kps_h;
   const uint8_t* vp = a.vp + b * a.vps_b + kvh * a.vps_h;
   const int64_t ks0 = b * a.kss_b + kvh * a.kss_h, vs0 = b * a.vss_b + kvh * a.vss_h;
-  const int word = tid % words, part = tid / words, parts = kRowThreads / words;
+  const int word = tid % words, part = tid / words, parts = NT / words;
   float m = -__builtin_inff(), l = 0.0f;
   float o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t j0 = 0; j0 < len; j0 += kRowThreads) {
+  for (int64_t j0 = 0; j0 < len; j0 += NT) {
     const int64_t j = j0 + tid;
     bool on = j < len && (j < base || block_sees(a, b, i, j - base));
     int64_t r = -1;
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(kRowThreads) void block_rows8_kernel(const BlockArg
     if ((tid & 63) == 0) red[wave] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kRowThreads / 64; ++w) mx = fmaxf(mx, red[w]);
+    for (int w = 0; w < NT / 64; ++w) mx = fmaxf(mx, red[w]);
     const float m_new = fmaxf(m, mx);
     const float alpha = m == m_new ? 1.0f : exp2f(m - m_new);
     const float p = s == -__builtin_inff() ? 0.0f : exp2f(s - m_new);
@@ -250,13 +251,13 @@ __global__ __launch_bounds__(kRowThreads) void block_rows8_kernel(const BlockArg
     if (a.out && part < parts) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k] *= alpha;
-      for (int x0 = part; x0 < kRowThreads; x0 += 8 * parts) {
+      for (int x0 = part; x0 < NT; x0 += 8 * parts) {
         uint32_t w[8];
         float sc[8];
 #pragma unroll
         for (int y = 0; y < 8; ++y) {  // (a key without weight is not read)
           const int x = x0 + y * parts;
-          const float p8 = x < kRowThreads ? p_lds[x] : 0.0f;
+          const float p8 = x < NT ? p_lds[x] : 0.0f;
           w[y] = 0u;
           sc[y] = 0.0f;
           if (p8 != 0.0f) {
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(kRowThreads) void block_rows8_kernel(const BlockArg
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
           const int x = x0 + y * parts;
-          const float p8 = x < kRowThreads ? p_lds[x] : 0.0f;
+          const float p8 = x < NT ? p_lds[x] : 0.0f;
           if (p8 != 0.0f) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) o[k] = fmaf(p8, (float)((int)((w[y] >> (4 * k)) & 15u) - 8) * sc[y], o[k]);
@@ -285,12 +286,21 @@ __global__ __launch_bounds__(kRowThreads) void block_rows8_kernel(const BlockArg
   __syncthreads();
   l = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kRowThreads / 64; ++w) l += red[w];
+  for (int w = 0; w < NT / 64; ++w) l += red[w];
   if (a.stats && tid == 0)
     a.stats[stats_at(a, b, h, i)] = make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
-  if (a.out && tid < a.D) {
-    float x = 0.0f;
-    for (int y = 0; y < parts; ++y) x += o_lds[(y * words) * 8 + tid];
+  if (!a.out) return;
+  // dim d's parts: first every (NT / D)-th of them, then those sums
+  const int d = tid % a.D, first = tid / a.D, step = NT / a.D;
+  float x = 0.0f;
+  if (first < step)
+    for (int y = first; y < parts; y += step) x += o_lds[(y * words) * 8 + d];
+  __syncthreads();
+  if (first < step) o_lds[tid] = x;
+  __syncthreads();
+  if (tid < a.D) {
+    x = 0.0f;
+    for (int y = 0; y < step; ++y) x += o_lds[y * a.D + tid];
     store_from_f32(a.out, b * a.os_b + h * a.os_h + i * a.os_s + tid * a.os_d, a.q_dt, l > 0.0f ? x / l : 0.0f);
   }
 }
@@ -304,7 +314,12 @@ void launch_block_rows(const BlockArgs& a, hipStream_t st) {
   };
   if (a.D % 8 == 0 && a.G % 8 == 0 && a.D % a.G == 0 && words(a.kp, a.kps_b, a.kps_h, a.kps_s) &&
       words(a.vp, a.vps_b, a.vps_h, a.vps_s))
-    hipLaunchKernelGGL(block_rows8_kernel, dim3((unsigned)n), dim3(kRowThreads), 0, st, a);
+    // 1024 keys at a time while all rows' workgroups are resident together (512):
+    // latency counts (fp32, 96 rows of 64 dims: 1000 keys 12.8 against 23.0 us,
+    // 4096 keys 32 against 78). More rows fill the GPU with 256 threads each (1536
+    // rows, 1000 keys: 54 against 71 us).
+    if (a.Sk > kRowThreads && n <= 512) hipLaunchKernelGGL((block_rows8_kernel<1024>), dim3((unsigned)n), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((block_rows8_kernel<256>), dim3((unsigned)n), dim3(256), 0, st, a);
   else
     hipLaunchKernelGGL(block_rows_kernel, dim3((unsigned)n), dim3(kRowThreads), 0, st, a);
 }
