@@ -474,7 +474,8 @@ int kvq_tree_attn_paged(const void* q, int q_dtype, const int64_t* q_strides,
  * sequence's length keep theirs. kvq_attn_key_weights also writes the block's
  * attention to out. Causal blocks align bottom-right, as kvq_decode_attn. No
  * reference counterpart. The sums' order is fixed (no atomics). A row that
- * attends no key, or whose softmax is not finite, adds nothing.
+ * attends no key adds nothing; a score that is NaN weighs nothing, infinite
+ * ones count as the largest (or smallest) of the row.
  * workspace: kvq_key_weights_workspace_bytes of uninitialised scratch, 16-byte
  * aligned (needed: KVQ_ESPACE without). Calls that overlap must not share it.
  */

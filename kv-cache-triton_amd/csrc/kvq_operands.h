@@ -190,7 +190,7 @@ __device__ __forceinline__ float query_operand(const uint16_t* p, bool vec, uint
   const uint32_t r0 = r[0], r1 = r[1];
   t = r0 > r1 ? r0 : r1;
   *odd = t >= (QF16 ? 0x7c00u : 0x7f80u);
-  const float u = unit_of(QF16 ? f16_bits_to_f32(t) : bf16_bits_to_f32(t));
+  const float u = *odd ? 1.0f : unit_of(QF16 ? f16_bits_to_f32(t) : bf16_bits_to_f32(t));
   const float un = qneg ? -u : u;
 #pragma unroll 1
   for (int kk = 0; kk < KS; ++kk) {

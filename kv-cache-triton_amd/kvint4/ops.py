@@ -1219,7 +1219,8 @@ def add_key_weights(
     weights that the queries q [B, Hq, Sq, D] give each cached key, summed over
     the KV head's query heads and the Sq rows: what an eviction ranks keys by.
     Causal blocks align bottom-right. Keys past seq_lens[b] keep their sum; a
-    row that attends no key, or whose softmax is not finite, adds nothing."""
+    row that attends no key adds nothing, and a score that is NaN weighs
+    nothing."""
     what = "add_key_weights"
     _check_block(what, q, q, k_packed, k_scales, key_weights)
     B, Hq, Sq, D = q.shape
@@ -1265,7 +1266,8 @@ def attention_with_key_weights(
     _check_weights(what, key_weights, B, n_kv_heads, Sk)
     # long blocks that the kernel with both does not take on the matrix cores:
     # the prefill kernels, and the weights beside them
-    matrix = D in (64, 128) and group_size in (32, 64, 128) and torch.float32 not in (q.dtype, k_scales.dtype)
+    matrix = (D in (64, 128) and group_size in (32, 64, 128) and D % group_size == 0
+              and torch.float32 not in (q.dtype, k_scales.dtype))
     if not matrix and seq_lens is None and use_prefill_kernel(Hq // n_kv_heads * Sq, Sk):
         try:
             prefill_attention(q, k_packed, k_scales, v_packed, v_scales, n_kv_heads=n_kv_heads, group_size=group_size,

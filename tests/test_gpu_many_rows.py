@@ -221,3 +221,32 @@ def test_two_graphs_of_wide_blocks_share_no_workspace():
             out.zero_()
             run()
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("s_dt", ["bf16", "f16"])
+def test_rows_that_are_not_finite_leave_the_sums_of_others(s_dt):
+    """A query of infinities and one of NaN: their blocks' other rows, and the weights of all, stay finite and bounded."""
+    g = torch.Generator().manual_seed(9)
+    B, Hq, Hkv, D, G, Sq, S, dt = 1, 4, 1, 128, 32, 40, 300, DT[s_dt]
+    cache = [t for _ in range(2) for t in random_cache(B, Hkv, S, D, G, dt, g, DEV)]
+    q = torch.randn(B, Hq, Sq, D, generator=g).to(dt).to(DEV)
+    kw = dict(n_kv_heads=Hkv, group_size=G, is_causal=False, sm_scale=D ** -0.5)
+    ref = Reference(q, values(*cache[:2], G, D), values(*cache[2:], G, D),
+                    allowed("none", [S], Sq, S, None, DEV), kw["sm_scale"])
+    q[:, 1, 7, 3] = math.inf
+    q[:, 2, 30] = math.nan
+    rows = [i for i in range(Sq) if i not in (7, 30)]
+    fine = ref.p[:, :, rows].sum((1, 2))  # [B, S]: the finite rows' weights
+    fine += ref.p[:, [0, 2, 3]][:, :, 7].sum(1) + ref.p[:, [0, 1, 3]][:, :, 30].sum(1)
+    for with_out in (False, True):
+        w = torch.zeros(B, Hkv, S, device=DEV)
+        if with_out:
+            out = ops.attention_with_key_weights(q, *cache, w, **kw)
+            err, tol = (out.double() - ref.out).abs()[:, :, rows], ref.tolerance(dt, STEP)[:, :, rows]
+            assert bool((err <= tol).all())
+        else:
+            ops.add_key_weights(q, cache[0], cache[1], w, **kw)
+        assert torch.isfinite(w).all()
+        more = w.double()[:, 0] - fine  # what the row of infinities adds: at most 1 in all, the row of NaN nothing
+        slack = ref.weight_tolerance(Hq * Sq, torch.zeros_like(ref.weights))[:, 0]
+        assert bool((more >= -slack).all()) and bool((more.sum(-1) <= 1 + slack.sum(-1) + 1e-6).all())
