@@ -321,31 +321,45 @@ void key_sums_kernel(const SumArgs a) {
   };
   load(lo);
 
-  // this wave's keys as the A operand
+  // this wave's keys as the A operand, times the power of two of the key with
+  // the largest scale; keys that fp16 would not hold so take their own, and the
+  // rare path their difference
   const uint8_t* kp = a.b.kp + b * a.b.kps_b + kvh * a.b.kps_h;
   const uint16_t* ks = (const uint16_t*)a.b.ks + b * a.b.kss_b + kvh * a.b.kss_h;
   uint4 k[KB][(TWO ? 2 : 1) * KS];
-  float back[KB][16];  // register j of a block: key 8 (j / 4) + 4 g + j % 4
+  float back[KB][16];  // of register j of a block: key 8 (j / 4) + 4 g + j % 4
   bool odd_k = false;
   const int kw = k0 + wave * 32 * KB;
+  uint64_t sraw[KB];
+  float u[KB], u_wave = 0x1p100f;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    sraw[kb] = load_scale_row(ks + min((int64_t)kw + 32 * kb + n, (int64_t)len - 1) * a.ng, a.ng);
+    u[kb] = key_unit(sraw[kb], a.ng, a.s_f16, &odd_k);
+    u_wave = fminf(u_wave, u[kb]);
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) u_wave = fminf(u_wave, __shfl_xor(u_wave, d));
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     const int64_t j = min((int64_t)kw + 32 * kb + n, (int64_t)len - 1);
-    const uint64_t sraw = load_scale_row(ks + j * a.ng, a.ng);
-    const float u = key_unit(sraw, a.ng, a.s_f16, &odd_k);
+    const bool far = u_wave < u[kb] * 0x1p-13f;
+    odd_k = odd_k || far;
+    const float uk = far ? u[kb] : u_wave;
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
       const uint32_t w = *(const uint32_t*)(kp + j * (D / 2) + 4 * (2 * kk + g));
-      const _Float16 s = (_Float16)(scale_at(sraw, 16 * kk / a.b.G, a.s_f16) * u);
+      const _Float16 s = (_Float16)(scale_at(sraw[kb], 16 * kk / a.b.G, a.s_f16) * uk);
       uint4 rest;
       k[kb][kk] = decode<TWO, !TWO>(w, s, &rest);
       if constexpr (TWO) k[kb][KS + kk] = rest;
     }
-    const float ub = 1.0f / u;
+    const float ub = u_wave / uk;
 #pragma unroll
     for (int x = 0; x < 16; ++x) back[kb][x] = __shfl(ub, 8 * (x >> 2) + 4 * g + (x & 3));
   }
   odd_k = __builtin_amdgcn_ballot_w64(odd_k) != 0;
+  const float back_wave = 1.0f / u_wave;
 
   float sum[KB][16];
 #pragma unroll
@@ -363,19 +377,17 @@ void key_sums_kernel(const SumArgs a) {
   for (int x = 0; x < 16; ++x) s_old[x] = -__builtin_inff();
   float4 r_old = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
   bool rare_old = false;
-  // scores that are not finite, and keys that a row does not attend, of keys k_first ..
+  // scores that are not finite or of keys with units of their own, and keys that
+  // a row does not attend, of keys k_first ..
   auto rare = [&](f32x16_t& s, const float (&bk)[16], float lim, int k_first) {
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      float u = bk[x];
-      asm volatile("" : "+v"(u));  // (nothing of the rare path is computed ahead, in registers of the loop)
-      const float inv = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, u));
-      s[x] = fminf(block_score(s[x] * u) * inv, 3.0e38f);
+      s[x] = block_score(s[x] * bk[x]);
       if (k_first + 8 * (x >> 2) + 4 * g + (x & 3) >= __builtin_bit_cast(int, lim)) s[x] = -__builtin_inff();
     }
   };
-  auto weigh = [&](const f32x16_t& s, const float (&bk)[16], const float4& r, float (&to)[16], int x) {
-    to[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x] * bk[x], r.z, -r.x)), r.y, to[x]);
+  auto weigh = [&](const f32x16_t& s, const float4& r, float (&to)[16], int x) {
+    to[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], r.z, -r.x)), r.y, to[x]);
   };
 #pragma unroll 1
   for (int t = lo; t < hi; ++t) {
@@ -405,20 +417,21 @@ void key_sums_kernel(const SumArgs a) {
         s = mfma(k[kb][TWO && x % 2 == 1 ? KS + kk : kk], f[kk & 1], s);
 #pragma unroll
         for (int y = 0; y < 16 / NM; ++y) {
-          weigh(s_old, back[kb_old], r_old, sum[kb_old], x * (16 / NM) + y);
+          weigh(s_old, r_old, sum[kb_old], x * (16 / NM) + y);
           asm volatile("" : "+v"(sum[kb_old][x * (16 / NM) + y]));  // (here, not where the sums are next read)
         }
         __builtin_amdgcn_sched_barrier(0);
       }
       s_old = s;
       r_old = row_lds[cur][32 * rb + n];
+      r_old.z *= back_wave;
       rare_old = odd_cur || kw + 32 * (kb + 1) > lim_tile;
     }
     __syncthreads();
   }
   if (rare_old) rare(s_old, back[KB - 1], r_old.w, kw + 32 * (KB - 1));
 #pragma unroll
-  for (int x = 0; x < 16; ++x) weigh(s_old, back[KB - 1], r_old, sum[KB - 1], x);
+  for (int x = 0; x < 16; ++x) weigh(s_old, r_old, sum[KB - 1], x);
   // over the 32 lanes of a key's rows
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)

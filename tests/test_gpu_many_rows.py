@@ -250,3 +250,27 @@ def test_rows_that_are_not_finite_leave_the_sums_of_others(s_dt):
         more = w.double()[:, 0] - fine  # what the row of infinities adds: at most 1 in all, the row of NaN nothing
         slack = ref.weight_tolerance(Hq * Sq, torch.zeros_like(ref.weights))[:, 0]
         assert bool((more >= -slack).all()) and bool((more.sum(-1) <= 1 + slack.sum(-1) + 1e-6).all())
+
+
+@pytest.mark.parametrize("far", FAR, ids=str)
+def test_weights_of_scales_far_apart(far):
+    g = torch.Generator().manual_seed(12)
+    B, Hq, Hkv, D, G, Sq, S = 1, 8, 2, 128, 32, 50, 400
+    cache = [t for _ in range(2) for t in random_cache(B, Hkv, S, D, G, torch.bfloat16, g, DEV)]
+    q = torch.randn(B, Hq, Sq, D, generator=g).bfloat16().to(DEV)
+    a, b, c = FAR[far]
+    f = cache[1].float() * 2.0 ** a
+    f[:, :, 100:140] = cache[1][:, :, 100:140].float() * 2.0 ** b
+    f[:, :, 200:220, 1] = cache[1][:, :, 200:220, 1].float() * 2.0 ** c
+    cache[1].copy_(f)
+    kw = dict(n_kv_heads=Hkv, group_size=G, is_causal=True, sm_scale=2.0 ** -max(a, b, c, 0) * 0.1)
+    ref = Reference(q, values(*cache[:2], G, D), values(*cache[2:], G, D), allowed("causal", [S], Sq, S, None, DEV),
+                    kw["sm_scale"])
+    for with_out in (False, True):
+        w = torch.zeros(B, Hkv, S, device=DEV)
+        if with_out:
+            _check(ops.attention_with_key_weights(q, *cache, w, **kw), ref, q.dtype)
+        else:
+            ops.add_key_weights(q, cache[0], cache[1], w, **kw)
+        err = (w.double() - ref.weights).abs()
+        assert bool((err <= ref.weight_tolerance(Hq // Hkv * Sq, torch.zeros_like(ref.weights))).all())
