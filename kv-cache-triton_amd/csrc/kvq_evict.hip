@@ -7,6 +7,11 @@
 // mapped to unsigned integers that compare as the floats do.
 // move: destination row first + i of each tensor is source row index[i].
 //
+// Measured: 8 heads of 16K rows cut to 2K 13.4 + 3.5 us, 400 heads of 1,100 rows
+// 11.5 + 9, 64 heads of 32K rows cut to 8K 23 + 50. The selection is bound by the
+// latency of its rounds (one workgroup per head), the move by memory: its rows
+// of 64 bytes of codes lie apart, and each fetches a line of 128.
+//
 // The reference's cache drops nothing (models/llama3/kv_cache.py:76-105).
 
 #include "kvq_common.h"

@@ -13,6 +13,12 @@
 //                      stay in registers, query tiles go through LDS
 //   key_add_kernel     the shares' sums to the running sums, in a fixed order
 //
+// Measured on a causal 4K prompt, 32 query heads over 8: key_sums_kernel 149 us
+// (461 TFLOP/s of scores; 246 when queries were converted in every workgroup and
+// products and exponentials took turns, 203 with the shares of the rows fixed),
+// row_stats_kernel 140, the additions 5. Bound by matrix cycles and exponentials,
+// which add up (256 and 450 cycles a 32 x 32 block).
+//
 // Scores are exact to fp32's rounding (kvq_operands.h). Both passes form them by
 // the same instructions in the same order, so that a row's weights add up to 1.
 //

@@ -4,12 +4,20 @@
 //                   of 2^(c s[i, j] - m[i]) / l[i],   c = log2 e,
 //                   m[i] = max_j c s[i, j],  l[i] = sum_j 2^(c s[i, j] - m[i])
 //
-// Both passes over the scores form them by the same operations in the same
-// order, so that the weights of a row add up to 1 however large its scores.
 // i.e. the softmax weights of a block of queries, summed over the rows that
 // share the KV head, added to a running fp32 sum per key: what an eviction
-// ranks the cache's rows by. Sums over rows are taken in a fixed order (no
-// atomics), so equal calls give equal bits. The reference has no counterpart.
+// ranks the cache's rows by. A key's sum needs every row's m and l, so the
+// scores are formed twice, by the same operations in the same order both times
+// (a row's weights then add up to 1 however large its scores), or kept:
+//   few rows with their attention   scores kept by kvq_block.hip
+//   other 16-bit blocks             kvq_rows.hip, then kvq_sums.hip
+//   the rest                        the plain kernels (the attention's, and below)
+// Sums over rows are taken in a fixed order (no atomics), so equal calls give
+// equal bits. The reference has no counterpart.
+//
+// Kept scores are 4 bytes a row and key, written and read: 134 MB for 8 sequences
+// of 32K keys and 64 heads (102 us in all). A second pass over that cache would
+// read as much and form the scores again.
 
 #include <algorithm>
 
