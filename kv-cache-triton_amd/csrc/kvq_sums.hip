@@ -13,8 +13,8 @@
 //                      stay in registers, query tiles go through LDS
 //   key_add_kernel     the shares' sums to the running sums, in a fixed order
 //
-// Measured on a causal 4K prompt, 32 query heads over 8: key_sums_kernel 149 us
-// (461 TFLOP/s of scores; 246 when queries were converted in every workgroup and
+// Measured on a causal 4K prompt, 32 query heads over 8: key_sums_kernel 139 us
+// (494 TFLOP/s of scores; 246 when queries were converted in every workgroup and
 // products and exponentials took turns, 203 with the shares of the rows fixed),
 // row_stats_kernel 140, the additions 5. Bound by matrix cycles and exponentials,
 // which add up (256 and 450 cycles a 32 x 32 block).
@@ -136,7 +136,7 @@ void row_stats_kernel(const SumArgs a) {
   auto store = [&](int buf) {
     bool odd = false;
     const float u = key_unit(sraw, a.ng, a.s_f16, &odd);
-    const _Float16 s = (_Float16)(scale_at(sraw, part * (8 * KP) / a.b.G, a.s_f16) * u);
+    const _Float16 s = (_Float16)(scale_at(sraw, part * (8 * KP) * a.ng / D, a.s_f16) * u);
 #pragma unroll
     for (int j = 0; j < KP; ++j) {  // dims 8 (KP part + j) .. + 7: step (KP part + j) / 2, half j % 2
       const int piece = KP * part + j;
@@ -336,35 +336,55 @@ void key_sums_kernel(const SumArgs a) {
   float back[KB][16];  // of register j of a block: key 8 (j / 4) + 4 g + j % 4
   bool odd_k = false;
   const int kw = k0 + wave * 32 * KB;
-  uint64_t sraw[KB];
-  float u[KB], u_wave = 0x1p100f;
+  // (no branches and few instructions: this runs once per workgroup, and straight
+  // code waits for its instructions)
+  constexpr int NC = D / 32;
+  float sc[KB][NC], u[KB], u_wave = 0x1p100f;
+  uint32_t w[KB][KS];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    sraw[kb] = load_scale_row(ks + min((int64_t)kw + 32 * kb + n, (int64_t)len - 1) * a.ng, a.ng);
-    u[kb] = key_unit(sraw[kb], a.ng, a.s_f16, &odd_k);
+    const int64_t j = min((int64_t)kw + 32 * kb + n, (int64_t)len - 1);
+    uint32_t bits[NC], top = 0u;
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc) bits[cc] = ks[j * a.ng + cc * a.ng / NC];
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) w[kb][kk] = *(const uint32_t*)(kp + j * (D / 2) + 4 * (2 * kk + g));
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc) {
+      top = max(top, bits[cc] & 0x7fffu);
+      sc[kb][cc] = TWO ? f16_bits_to_f32(bits[cc]) : bf16_bits_to_f32(bits[cc]);
+    }
+    const bool odd = top >= (TWO ? 0x7c00u : 0x7f80u);  // (a key that is not finite: the unit 1)
+    odd_k |= odd;
+    u[kb] = odd ? 1.0f : unit_of(TWO ? f16_bits_to_f32(top) : bf16_bits_to_f32(top));
     u_wave = fminf(u_wave, u[kb]);
   }
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) u_wave = fminf(u_wave, __shfl_xor(u_wave, d));
+  bool any_far = false;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    const int64_t j = min((int64_t)kw + 32 * kb + n, (int64_t)len - 1);
     const bool far = u_wave < u[kb] * 0x1p-13f;
-    odd_k = odd_k || far;
-    const float uk = far ? u[kb] : u_wave;
+    any_far |= far;
+    u[kb] = far ? u[kb] : u_wave;
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
-      const uint32_t w = *(const uint32_t*)(kp + j * (D / 2) + 4 * (2 * kk + g));
-      const _Float16 s = (_Float16)(scale_at(sraw[kb], 16 * kk / a.b.G, a.s_f16) * uk);
       uint4 rest;
-      k[kb][kk] = decode<TWO, !TWO>(w, s, &rest);
+      k[kb][kk] = decode<TWO, !TWO>(w[kb][kk], (_Float16)(sc[kb][kk / 2] * u[kb]), &rest);
       if constexpr (TWO) k[kb][KS + kk] = rest;
     }
-    const float ub = u_wave / uk;
 #pragma unroll
-    for (int x = 0; x < 16; ++x) back[kb][x] = __shfl(ub, 8 * (x >> 2) + 4 * g + (x & 3));
+    for (int x = 0; x < 16; ++x) back[kb][x] = 1.0f;
   }
-  odd_k = __builtin_amdgcn_ballot_w64(odd_k) != 0;
+  if (__builtin_amdgcn_ballot_w64(any_far) != 0) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const float ub = u_wave / u[kb];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) back[kb][x] = __shfl(ub, 8 * (x >> 2) + 4 * g + (x & 3));
+    }
+  }
+  odd_k = __builtin_amdgcn_ballot_w64(odd_k | any_far) != 0;
   const float back_wave = 1.0f / u_wave;
 
   float sum[KB][16];
@@ -438,17 +458,26 @@ void key_sums_kernel(const SumArgs a) {
   if (rare_old) rare(s_old, back[KB - 1], r_old.w, kw + 32 * (KB - 1));
 #pragma unroll
   for (int x = 0; x < 16; ++x) weigh(s_old, r_old, sum[KB - 1], x);
-  // over the 32 lanes of a key's rows
+  // over the 32 lanes of a key's rows: at each step a lane passes on half of its
+  // keys and takes the other half's sums, so that lane n ends with key n's
+  float v[16 * KB];
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
+  for (int x = 0; x < 16 * KB; ++x) v[x] = sum[x / 16][x % 16];
+  int d = 16;
 #pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      float v = sum[kb][x];
+  for (int half = 8 * KB; half >= 1; half /= 2) {
+    const bool up = (n & d) != 0;
 #pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-      const int key = kw + 32 * kb + 8 * (x >> 2) + 4 * g + (x & 3);
-      if (n == 0 && key < len) dst[key] = v;
+    for (int x = 0; x < half; ++x) {
+      const float mine = up ? v[x + half] : v[x], other = up ? v[x] : v[x + half];
+      v[x] = mine + __shfl_xor(other, d);
     }
+    d /= 2;
+  }
+  if constexpr (KB == 1) v[0] += __shfl_xor(v[0], 1);
+  const int e = KB == 1 ? n >> 1 : n;  // block e / 16, register e % 16
+  const int key = kw + 32 * (e >> 4) + 8 * ((e & 15) >> 2) + 4 * g + (e & 3);
+  if (key < len && (KB == 2 || n % 2 == 0)) dst[key] = v[0];
 }
 
 // A thread a key: memory-bound.
