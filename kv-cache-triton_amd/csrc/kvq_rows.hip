@@ -85,27 +85,11 @@ void rows_attn_kernel(const RowsArgs a) {
   const int lo = (int)((uint32_t)tiles * (uint32_t)sp / (uint32_t)a.m.n_split);
   const int hi = (int)((uint32_t)tiles * (uint32_t)(sp + 1) / (uint32_t)a.m.n_split);
 
-  // ---- queries: lane (n, g) holds dims 16 kk + 8 g .. + 7 of its row ----
   const int R0 = blk * ROWS + wave * 32, R = R0 + n;
   const int row_i = min(R, rows - 1) / ab.ratio, head = kvh * ab.ratio + (min(R, rows - 1) - row_i * ab.ratio);
   // keys that every row of the wave attends
   int lim_wave = R0 < rows ? limit(R0 / ab.ratio) : 0x7fffffff;
   if (ab.kind == kMaskTree) lim_wave = min(lim_wave, max(base, 0));
-  uint4 q[KS];
-  float cr, q_unit;
-  bool q_odd = false;
-  {
-    const uint16_t* p = (const uint16_t*)ab.q + b * ab.qs_b + (int64_t)head * ab.qs_h + (int64_t)row_i * ab.qs_s + 8 * g;
-    q_unit = query_operand<QF16, KS>(p, a.m.q_vec, ab.scale_log2 < 0.0f, q, &q_odd);
-    q_odd = __builtin_amdgcn_ballot_w64(q_odd) != 0;
-    if (SUMS && sp == 0 && R0 < rows) {
-      const int64_t block = (int64_t)unit * a.qi.blocks + R0 / 32;
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk) a.qi.img[(block * KS + kk) * 64 + lane] = q[kk];
-      if (lane == 0) a.qi.odd[block] = q_odd;
-      if (g == 0 && R < rows) a.qi.unit[(int64_t)unit * rows + R] = q_unit;
-    }
-  }
 
   // ---- tiles: first cache row and rows of tile t ----
   const uint8_t* kp = ab.kp + b * ab.kps_b + kvh * ab.kps_h;
@@ -230,6 +214,27 @@ void rows_attn_kernel(const RowsArgs a) {
     load_keys(r0_cur, nr_cur);
     load_v_scales(r0_cur, nr_cur);
     load_values(r0_cur, nr_cur);
+  }
+
+  // ---- queries (on their way with the first tile): lane (n, g) holds dims
+  // 16 kk + 8 g .. + 7 of its row ----
+  uint4 q[KS];
+  float cr, q_unit;
+  bool q_odd = false;
+  {
+    const uint16_t* p = (const uint16_t*)ab.q + b * ab.qs_b + (int64_t)head * ab.qs_h + (int64_t)row_i * ab.qs_s + 8 * g;
+    q_unit = query_operand<QF16, KS>(p, a.m.q_vec, ab.scale_log2 < 0.0f, q, &q_odd);
+    q_odd = __builtin_amdgcn_ballot_w64(q_odd) != 0;
+    if (SUMS && sp == 0 && R0 < rows) {
+      const int64_t block = (int64_t)unit * a.qi.blocks + R0 / 32;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) a.qi.img[(block * KS + kk) * 64 + lane] = q[kk];
+      if (lane == 0) a.qi.odd[block] = q_odd;
+      if (g == 0 && R < rows) a.qi.unit[(int64_t)unit * rows + R] = q_unit;
+    }
+  }
+
+  if (lo < hi) {
     {  // the powers of two of the scales, from the first tile's
       float tk = fabsf(scale_f32(ks_raw)), tv = fabsf(scale_f32(vs_raw));
       tk = tk < __builtin_inff() ? tk : 0.0f;
