@@ -506,7 +506,8 @@ SumPlan sum_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64
   p.key_blocks = (Sk + keys - 1) / keys;
   // shares of the rows: the number of them with the least estimate, in tiles'
   // times: rounds of the 512 workgroups that are resident together, each its
-  // tiles and about three tiles' time of prologue
+  // tiles and about three tiles' time of prologue (4K prompt with its attention:
+  // 12 shares 315 us, 16 323, 20, the estimate's, 303, 32 324, 48 332)
   const int64_t tiles = (rows + kTile - 1) / kTile, ratio = Hq / Hkv;
   double best = 0.0;
   p.chunks = p.chunk_tiles = 0;
